@@ -240,6 +240,137 @@ void sdy_p2p_clear_status(void);
 int sdy_qmatvec_f32_noalloc(const void *w, const float *d_x, int n_tok, float *d_out, int64_t ldo, int64_t row0,
                             int64_t row1, void *stream);
 
+/* ------------------------------------------------------------------ drafted-token steps
+ *
+ * No counterpart in the reference, which decodes one token of one sequence at a time. The three
+ * operators that a step of speculative decoding needs around the products: rotary positions with
+ * the KV store, attention of a tree of drafted tokens over the cache, and sampling. Each takes its
+ * arguments in a block that the caller keeps and may reuse; data pointers are DEVICE pointers of
+ * the current device (or pinned host memory mapped there) that the caller owns. Calls are
+ * asynchronous on `stream`, take no memory of their own, can be captured into a graph, and return
+ * 0 or -1 (sdy_last_error). `type` is F32 0, F16 1 or BF16 30 and holds for every value pointer of
+ * the block; strides count elements. Counts of zero are valid and launch nothing. */
+
+/* Frequencies of rotary positions. Pair i of n_rot/2 turns by theta^(-2i/n_rot) radians per
+ * position, divided by factors[i] when `factors` is set, then scaled for contexts longer than the
+ * trained orig_ctx positions:
+ *   0  not at all (factor, low, high, orig_ctx ignored);
+ *   1  linearly: divided by `factor`;
+ *   2  by wavelength: kept where orig_ctx holds more than `high` turns, divided by `factor` where it
+ *      holds fewer than `low`, and mixed linearly in the number of turns between the two;
+ *   3  by dimension: the same mix, linear in the pair's index between the pairs that make `high` and
+ *      `low` turns over orig_ctx (rounded outwards to whole indexes of the n_rot dimensions). */
+typedef struct {
+    int32_t n_rot, scaling, orig_ctx, reserved;
+    double theta, factor, low, high;
+    const float *factors; /* host, n_rot/2 values, or NULL */
+} sdy_rope_spec;
+/* Writes n_rot/2 radians per position to `freq` (host). 0 or -1. Needs no GPU. */
+int sdy_rope_freqs(const sdy_rope_spec *spec, double *freq);
+
+/* Rotates the first n_rot elements of every query and key head of n_tok tokens by pos[t] * freq[i]
+ * and multiplies them by mscale (1 unless the scaling asks for another magnitude); the other
+ * elements are copied. Pairs are (i, i + n_rot/2), or (2i, 2i+1) when `interleaved`. Angles are
+ * formed in 64 bits, the rotation in 32, rounded once.
+ *
+ * Queries go to q_out (which may be q itself with the same strides). Keys go to row
+ * slot[t] % max_seq of sequence slot[t] / max_seq of k_cache, and v, when set, unrotated to the
+ * same row of v_cache: element e of head h at seq*cache_seq + h*cache_head + row*cache_row + e.
+ * slot NULL means slot[t] = t. A slot outside [0, n_seq*max_seq) stores nothing (padding tokens).
+ * Slots must differ: of two tokens with one slot, the row holds a mixture. n_head 0 leaves out the
+ * queries, n_kv_head 0 the keys and values. Other overlaps of inputs and outputs are not allowed. */
+typedef struct {
+    int32_t type, n_tok, n_head, n_kv_head;
+    int32_t head_dim;    /* 1..1024 */
+    int32_t n_rot;       /* even, 0..head_dim */
+    int32_t interleaved;
+    float mscale;
+    const double *freq;  /* device, n_rot/2 radians per position (sdy_rope_freqs) */
+    const int32_t *pos;  /* device, n_tok */
+    const void *q;
+    int64_t q_tok, q_head;
+    void *q_out;
+    int64_t q_out_tok, q_out_head;
+    const void *k;
+    int64_t k_tok, k_head;
+    const void *v;       /* or NULL */
+    int64_t v_tok, v_head;
+    void *k_cache, *v_cache;
+    const int64_t *slot; /* device, n_tok, or NULL */
+    int64_t n_seq, max_seq, cache_seq, cache_head, cache_row;
+} sdy_rope_args;
+int sdy_rope_dev(const sdy_rope_args *a, void *stream);
+
+/* Attention of drafted tokens over a KV cache. Sequence s has n_past[s] cached tokens in rows
+ * [0, n_past[s]) and its n_node drafted ones behind them, node i in row n_past[s] + i. parent[s][i]
+ * is -1 for a node that continues the sequence, or an earlier node (0 <= parent < i); any other
+ * value marks a padding node, as does a path that ends in one. parent NULL: a chain (parent i-1).
+ * Node i sees every cached row and the rows of its own path (itself included):
+ *   out[s][i][h] = sum_j p_j v_j,  p = softmax over the rows it sees of scale * (q . k_j),
+ * with KV head h / (n_head / n_kv_head). A padding node's output is zero, and its K and V rows are
+ * not read by any other: what rows a node does not see hold (NaN, infinities) does not matter. Rows
+ * from max_seq on do not exist (a negative n_past counts as 0). Scores, softmax statistics and
+ * sums are held in 32 bits; 16-bit caches are multiplied on the tensor cores with the
+ * probabilities rounded to the cache's type. The order of the sums does not depend on timing:
+ * the same call gives the same bits.
+ *
+ * n_node 1..256 (1: plain decoding), n_head a multiple of n_kv_head, head_dim a multiple of 8 up to
+ * 256, every pointer 16-byte aligned, strides multiples of 16 bytes. `ws`: sdy_tree_attention_bytes
+ * (which reads the counts and max_seq alone) bytes of device memory that no other call uses while
+ * this one runs; nothing needs clearing. */
+typedef struct {
+    int32_t type, n_seq, n_node, n_head, n_kv_head, head_dim, max_seq;
+    float scale;
+    const void *q;
+    int64_t q_seq, q_node, q_head;
+    const void *k_cache, *v_cache;
+    int64_t cache_seq, cache_head, cache_row;
+    const int32_t *n_past;  /* device, n_seq */
+    const int32_t *parent;  /* device, n_seq * n_node, or NULL */
+    void *out;              /* not q */
+    int64_t out_seq, out_node, out_head;
+    void *ws;
+    size_t ws_bytes;
+} sdy_tree_attention_args;
+size_t sdy_tree_attention_bytes(const sdy_tree_attention_args *a); /* 0 on error */
+int sdy_tree_attention_dev(const sdy_tree_attention_args *a, void *stream);
+
+/* Samples one token per row of logits. With w_i = exp((logit_i - max) / temperature):
+ *   top_k > 0:       only the top_k largest logits are kept;
+ *   top_p in [0,1):  of those, in descending order, the shortest prefix whose share of their sum
+ *                    reaches top_p (at least one);
+ *   min_p > 0:       of those, the ones with w_i >= min(min_p, 1), i.e. at least min_p times as
+ *                    likely as the largest;
+ * equal logits rank by index, the lowest first. The token is the first kept index at which the
+ * running sum of w over the kept indexes, in index order, exceeds u times the whole sum; u is
+ * clamped to [0, 1) and NaN counts as 0. prob is its share of the sum. A temperature that is not
+ * positive (NaN included) takes the largest logit, prob 1. NaN and -inf logits are never taken; +inf
+ * ones share the whole weight; a row without any other gives id -1 and prob 0. NaN parameters switch
+ * their filter off. The weights are computed in 64 bits and their sums taken over whole multiples
+ * of 2^-44 (one that rounds to none, below 2^-45 of the largest, has no share), so neither the
+ * launch shape nor timing changes a choice.
+ * n_vocab 1..400000. Parameter arrays (device, one value per row) may be NULL: temperature 1, the
+ * filter off. */
+typedef struct {
+    int32_t type, n_row, n_vocab, reserved;
+    int64_t row_stride;
+    const void *logits;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    const float *u;     /* device, one uniform number in [0, 1) per row */
+    int32_t *id;        /* device, n_row */
+    float *prob;        /* device, n_row, or NULL */
+} sdy_sample_args;
+int sdy_sample_dev(const sdy_sample_args *a, void *stream);
+
+/* engine_eval of `tokens`, then the token sampled on the device from the last token's logits as
+ * sdy_sample_dev does (one row, these parameters) into *next; no logits are copied to the host
+ * (engine_logits returns NULL until the next engine_eval). Same errors as engine_eval, and a row
+ * without any finite or +inf logit is one. 0 or -1. */
+int sdy_engine_eval_sample(engine_ctx *c, const int32_t *tokens, int32_t n, float temperature, int32_t top_k,
+                           float top_p, float min_p, float u, int32_t *next);
+
 #ifdef __cplusplus
 }
 #endif

@@ -40,6 +40,32 @@ class EngineModelInfo(ctypes.Structure):
                                                     "n_expert", "n_expert_used", "ffn_exp_dim")]
 
 
+# The argument blocks of the drafted-token operators (include/sardyne_b200.h).
+def _fields(text):
+    kinds = {"i": _i32, "l": ctypes.c_int64, "f": ctypes.c_float, "d": ctypes.c_double, "p": _vp, "z": _sz}
+    return [(name, kinds[kind]) for kind, names in (part.split(":") for part in text.split(";")) for name in names.split()]
+
+
+class RopeSpec(ctypes.Structure):
+    _fields_ = _fields("i:n_rot scaling orig_ctx reserved;d:theta factor low high;p:factors")
+
+
+class RopeArgs(ctypes.Structure):
+    _fields_ = _fields("i:type n_tok n_head n_kv_head head_dim n_rot interleaved;f:mscale;p:freq pos q;l:q_tok q_head;"
+                       "p:q_out;l:q_out_tok q_out_head;p:k;l:k_tok k_head;p:v;l:v_tok v_head;p:k_cache v_cache slot;"
+                       "l:n_seq max_seq cache_seq cache_head cache_row")
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    _fields_ = _fields("i:type n_seq n_node n_head n_kv_head head_dim max_seq;f:scale;p:q;l:q_seq q_node q_head;"
+                       "p:k_cache v_cache;l:cache_seq cache_head cache_row;p:n_past parent out;"
+                       "l:out_seq out_node out_head;p:ws;z:ws_bytes")
+
+
+class SampleArgs(ctypes.Structure):
+    _fields_ = _fields("i:type n_row n_vocab reserved;l:row_stride;p:logits temperature top_k top_p min_p u id prob")
+
+
 # The reference's exported surface (sardyne/capi.py:33-102).
 SIGNATURES = {
     "engine_version": (ctypes.c_char_p, []),
@@ -133,6 +159,13 @@ EXTENSIONS = {
     "sdy_p2p_read": (_i, [_vp, _vp, _sz]),
     "sdy_p2p_status": (ctypes.c_uint32, []),
     "sdy_p2p_clear_status": (None, []),
+    "sdy_rope_freqs": (_i, [ctypes.POINTER(RopeSpec), ctypes.POINTER(ctypes.c_double)]),
+    "sdy_rope_dev": (_i, [ctypes.POINTER(RopeArgs), _vp]),
+    "sdy_tree_attention_bytes": (_sz, [ctypes.POINTER(TreeAttentionArgs)]),
+    "sdy_tree_attention_dev": (_i, [ctypes.POINTER(TreeAttentionArgs), _vp]),
+    "sdy_sample_dev": (_i, [ctypes.POINTER(SampleArgs), _vp]),
+    "sdy_engine_eval_sample": (_i, [_vp, ctypes.POINTER(_i32), _i32, ctypes.c_float, _i32, ctypes.c_float,
+                                    ctypes.c_float, ctypes.c_float, ctypes.POINTER(_i32)]),
     "sdy_qmatvec_f32_noalloc": (_i, [_vp, _vp, _i, _vp, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _vp]),
 }
 

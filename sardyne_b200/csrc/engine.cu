@@ -11,6 +11,7 @@
 #include "common.cuh"
 #include "fp_ops.cuh"
 #include "fused.cuh"
+#include "sample.cuh"
 #include "sardyne_b200.h"
 
 #include <dlfcn.h>
@@ -214,6 +215,7 @@ struct engine_ctx {
     int *am_i = nullptr;
     unsigned *am_count = nullptr;
     int32_t *am_out = nullptr, *h_am_out = nullptr;
+    SampleWords *sp = nullptr, *h_sp = nullptr;  // sampled choice: the call's parameters, device and pinned
     unsigned *h_md_status = nullptr;  // pinned copy of the status word, read after each eval
     int32_t *grp_off = nullptr, *grp_slot = nullptr, *grp_tiles = nullptr;  // slots by expert (prefill GEMM)
     // Sharded models: all-reduce sources, zero outside this rank's columns (hsend: FFN activations
@@ -1551,6 +1553,7 @@ engine_ctx *engine_ctx_new(const engine_model *m, int32_t max_seq, int32_t n_bat
         {(void **)&c->tokpos, (B + 1) * 4},
         {(void **)&c->am_v, ARGMAX_CTAS * 4}, {(void **)&c->am_i, ARGMAX_CTAS * 4},
         {(void **)&c->am_count, 4}, {(void **)&c->am_out, 4},
+        {(void **)&c->sp, sizeof(SampleWords)},
     };
     if (in.n_expert) {
         items.push_back({(void **)&c->moe_probs, B * in.n_expert * 4});
@@ -1616,7 +1619,8 @@ engine_ctx *engine_ctx_new(const engine_model *m, int32_t max_seq, int32_t n_bat
                !SDY_CUDA(cudaMallocHost(&c->h_logits, lbytes)) || !SDY_CUDA(cudaMallocHost(&c->h_tokpos, (B + 1) * 4)) ||
                !SDY_CUDA(cudaMallocHost(&c->h_md_status, sizeof(unsigned))) ||
                !SDY_CUDA(cudaMallocHost(&c->h_px_status, sizeof(unsigned))) ||
-               !SDY_CUDA(cudaMallocHost(&c->h_am_out, sizeof(int32_t))))) {
+               !SDY_CUDA(cudaMallocHost(&c->h_am_out, sizeof(int32_t))) ||
+               !SDY_CUDA(cudaMallocHost(&c->h_sp, sizeof(SampleWords))))) {
         put_err(err, err_len, "inizializzazione del contesto fallita: %s", last_error());
         ok = false;
     }
@@ -1649,13 +1653,14 @@ void engine_ctx_free(engine_ctx *c) {
     if (c->h_tokpos) cudaFreeHost(c->h_tokpos);
     if (c->h_md_status) cudaFreeHost(c->h_md_status);
     if (c->h_am_out) cudaFreeHost(c->h_am_out);
+    if (c->h_sp) cudaFreeHost(c->h_sp);
     delete c;
 }
 
 namespace {
-// engine_eval, with the last token's greedy choice made on the device instead of the logits
-// copied back when `next` is set.
-int eval_tokens(engine_ctx *c, const int32_t *tokens, int32_t n, int32_t *next) {
+// engine_eval, with the last token's greedy choice, or with `how` the sampled one, made on the
+// device instead of the logits copied back when `next` is set.
+int eval_tokens(engine_ctx *c, const int32_t *tokens, int32_t n, int32_t *next, const SampleWords *how = nullptr) {
     if (!c) return -1;
     c->err[0] = '\0';
     if (!tokens || n < 1) {
@@ -1680,6 +1685,11 @@ int eval_tokens(engine_ctx *c, const int32_t *tokens, int32_t n, int32_t *next) 
         snprintf(c->err, sizeof c->err, "contesto inutilizzabile: uno scambio tra GPU era scaduto");
         return -1;
     }
+    if (how && c->m->info.n_vocab > SAMPLE_MAX_VOCAB) {
+        snprintf(c->err, sizeof c->err, "vocabolario di %d token: il campionamento ne ammette %d", c->m->info.n_vocab,
+                 SAMPLE_MAX_VOCAB);
+        return -1;
+    }
     cudaSetDevice(c->m->dev);
     clear_error();
     const int saved = c->n_past;
@@ -1694,7 +1704,24 @@ int eval_tokens(engine_ctx *c, const int32_t *tokens, int32_t n, int32_t *next) 
         done += chunk;
     }
     const int nv = c->m->info.n_vocab;
-    if (next) {
+    if (how) {
+        *c->h_sp = *how;
+        SDY_CUDA(cudaMemcpyAsync(c->sp, c->h_sp, sizeof(SampleWords), cudaMemcpyHostToDevice, c->st));
+        sdy_sample_args a = {};
+        a.type = T_F32;
+        a.n_row = 1;
+        a.n_vocab = nv;
+        a.row_stride = nv;
+        a.logits = c->logits + (size_t)(out_rows - 1) * nv;
+        a.temperature = &c->sp->temperature;
+        a.top_k = &c->sp->top_k;
+        a.top_p = &c->sp->top_p;
+        a.min_p = &c->sp->min_p;
+        a.u = &c->sp->u;
+        a.id = c->am_out;
+        sample_rows(a, c->st);
+        SDY_CUDA(cudaMemcpyAsync(c->h_am_out, c->am_out, 4, cudaMemcpyDeviceToHost, c->st));
+    } else if (next) {
         launch(argmax_kernel, ARGMAX_CTAS, ARGMAX_THREADS, 0, c->st, c->logits + (size_t)(out_rows - 1) * nv, nv,
                c->am_v, c->am_i, c->am_count, c->am_out);
         SDY_LAUNCHED();
@@ -1720,6 +1747,11 @@ int eval_tokens(engine_ctx *c, const int32_t *tokens, int32_t n, int32_t *next) 
         snprintf(c->err, sizeof c->err, "errore GPU: %s", last_error());
         return -1;
     }
+    if (how && *c->h_am_out < 0) {
+        c->n_past = saved;
+        snprintf(c->err, sizeof c->err, "nessun logit valido da campionare");
+        return -1;
+    }
     c->n_logits = next ? 0 : c->logits_all ? n : 1;
     if (next) *next = *c->h_am_out;
     return 0;
@@ -1734,6 +1766,16 @@ int sdy_engine_eval_greedy(engine_ctx *c, const int32_t *tokens, int32_t n, int3
         return -1;
     }
     return eval_tokens(c, tokens, n, next);
+}
+
+int sdy_engine_eval_sample(engine_ctx *c, const int32_t *tokens, int32_t n, float temperature, int32_t top_k,
+                           float top_p, float min_p, float u, int32_t *next) {
+    if (c && !next) {
+        snprintf(c->err, sizeof c->err, "sdy_engine_eval_sample: next NULL");
+        return -1;
+    }
+    const SampleWords how = {temperature, top_k, top_p, min_p, u};
+    return eval_tokens(c, tokens, n, next, &how);
 }
 
 const float *engine_logits(const engine_ctx *c) { return c && c->n_logits ? c->h_logits : nullptr; }
