@@ -6,6 +6,7 @@
 #include "common.cuh"
 #include "fp_ops.cuh"
 #include "sardyne_b200.h"
+#include "tree_attention.cuh"
 
 #include <stdarg.h>
 #include <string.h>
@@ -157,11 +158,12 @@ const char *engine_version(void) { return "0.0.1"; }
 const char *sdy_last_error(void) { return last_error(); }
 void sdy_clear_error(void) { clear_error(); }
 uint64_t sdy_kernel_launches(void) { return g_launches.load(); }
-uint32_t sdy_kernel_status(void) { return qgemm_status() | qmatvec_status(); }
+uint32_t sdy_kernel_status(void) { return qgemm_status() | qmatvec_status() | tree_tc_status(); }
 
 void sdy_kernel_clear_status(void) {
     qgemm_clear_status();
     qmatvec_clear_status();
+    tree_tc_clear_status();
 }
 
 static int g_simd = 1;
