@@ -7,15 +7,23 @@
 
 #include <algorithm>
 #include <initializer_list>
+#include <vector>
 
 namespace sdy {
 
 inline int value_bytes(int type) { return type == T_F32 ? 4 : 2; }
 
+// Ordinal of the device that the driver knows `p` to belong to (false: it knows no such memory).
+bool pointer_device(const void *p, int *device);
+
 // True when the kernels of the current device may use `p`: memory of that device, managed memory,
 // or pinned host memory mapped there. A pointer of another device or of pageable host memory would
 // fault in the kernel, so it is refused here.
+// (The driver's one-attribute query answers for memory of the current device in a fraction of the
+// full query's time; a call makes up to nine.)
 inline bool device_pointer(const char *fn, const char *name, const void *p) {
+    int at_device = -1, current = -1;
+    if (pointer_device(p, &at_device) && cudaGetDevice(&current) == cudaSuccess && at_device == current) return true;
     cudaPointerAttributes at;
     if (!SDY_CUDA(cudaPointerGetAttributes(&at, p))) return false;
     int dev = -1;
@@ -34,15 +42,13 @@ struct Axis {
 // True when the elements of an output with these axes above a contiguous run of `inner` elements
 // cannot coincide: each axis steps over all that the smaller ones span.
 inline bool disjoint(std::initializer_list<Axis> axes, int64_t inner) {
-    Axis a[4];
-    int n = 0;
-    for (const Axis &x : axes)
-        if (x.count > 1) a[n++] = x;
-    std::sort(a, a + n, [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+    std::vector<Axis> a(axes);
+    std::sort(a.begin(), a.end(), [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
     int64_t span = inner;
-    for (int i = 0; i < n; i++) {
-        if (a[i].stride < span || a[i].stride > (int64_t)1 << 48) return false;
-        span += a[i].stride * (a[i].count - 1);
+    for (const Axis &x : a) {
+        if (x.count <= 1) continue;
+        if (x.stride < span || x.stride > (int64_t)1 << 48) return false;
+        span += x.stride * (x.count - 1);
     }
     return true;
 }

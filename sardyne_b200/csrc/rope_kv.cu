@@ -14,6 +14,7 @@
 #include "draft.cuh"
 #include "sardyne_b200.h"
 
+#include <cuda.h>
 #include <math.h>
 
 namespace sdy {
@@ -185,6 +186,20 @@ void rope_launch(const sdy_rope_args &a, cudaStream_t s) {
 }
 
 }  // namespace
+
+bool pointer_device(const void *p, int *device) {
+    typedef CUresult (*Query)(void *, CUpointer_attribute, CUdeviceptr);
+    static const Query query = [] {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuPointerGetAttribute", &f, 12000, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return (Query)f;
+    }();
+    return query && query(device, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, (CUdeviceptr)p) == CUDA_SUCCESS;
+}
+
 }  // namespace sdy
 
 using namespace sdy;

@@ -85,57 +85,141 @@ __global__ void __launch_bounds__(32 * SIMPLE_WARPS) tree_simple_kernel(const sd
 }
 
 // The results of the row groups that the shares cut: out = sum_c f_c o_c / sum_c f_c l_c over the
-// CTAs that hold tiles of the group, in their order, with f_c = 2^(m_c - max m). One block per row
-// group and eight rows; a thread holds four elements of a row.
-constexpr int JOIN_ROWS = 8, JOIN_THREADS = 256;
+// CTAs that hold tiles of the group, in their order, with f_c = 2^(m_c - max m). A warp takes one row
+// of a cut group (two or four where rows are narrow), the warps of all SMs in turn: its lanes start the
+// copies of the first sixteen parts into shared memory (as many loads into registers the compiler
+// would not keep in flight), form the factors meanwhile, and add up four elements of a row each.
+// Bound by the latencies of the cuts, the maxima and the parts, one after the other (about 1 us each
+// on B200), and for many wide parts by what an SM reads from L2, 64 bytes a cycle.
+constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 16, JOIN_BLOCKS = 5 * TA_CTAS;
+constexpr int JOIN_FEW = 4;  // so many parts at most are loaded straight into registers
+constexpr int JOIN_RUNS = (TA_CTAS + 31) / 32;  // cuts, or parts, a lane looks at
+template <class T> __device__ __forceinline__ void store_quad(T *out, float4 v, float f) {
+    struct alignas(4 * sizeof(T)) Quad { T v[4]; } q;
+    q.v[0] = from_f32<T>(f == 0.0f ? 0.0f : v.x * f), q.v[1] = from_f32<T>(f == 0.0f ? 0.0f : v.y * f);
+    q.v[2] = from_f32<T>(f == 0.0f ? 0.0f : v.z * f), q.v[3] = from_f32<T>(f == 0.0f ? 0.0f : v.w * f);
+    *(Quad *)out = q;
+}
 template <class T>
-__global__ void __launch_bounds__(JOIN_THREADS)
-    join_kernel(const sdy_tree_attention_args p, const int64_t *base, const float4 *o, const float2 *ml, int rows_per_group,
-                int max_ctas) {
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+    join_kernel(const sdy_tree_attention_args p, const Cut *__restrict__ cuts, const float *__restrict__ o,
+                const float2 *__restrict__ ml, int rows_per_group) {
+    __shared__ float factor[JOIN_WARPS][4][TA_CTAS];
+    __shared__ int16_t active[JOIN_WARPS][TA_CTAS];
+    extern __shared__ float4 ahead[];  // [warps][JOIN_AHEAD][32]
     pdl_wait();
-    const int rep = p.n_head / p.n_kv_head, rows = p.n_node * rep;
-    const int groups = (rows + rows_per_group - 1) / rows_per_group, per_tile = p.n_kv_head * groups;
-    const int s = blockIdx.x / per_tile, kv = blockIdx.x % per_tile / groups, group = blockIdx.x % groups;
-    const int64_t units = base[p.n_seq] * per_tile, tiles = base[s + 1] - base[s], ctas = min((int64_t)max_ctas, units);
-    const int64_t u0 = base[s] * per_tile + (kv * groups + group) * tiles, u1 = u0 + tiles;
-    const int c0 = (int)(((u0 + 1) * ctas - 1) / units), c1 = (int)((u1 * ctas - 1) / units);
-    if (c0 == c1) return;  // written by the CTA that holds it
-    // the slot of CTA c's part: its share's first run, except where the group starts inside the share
-    const int first = units * c0 / ctas == u0 ? 0 : 1;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int in_group = blockIdx.y * JOIN_ROWS + lane / 4, row = group * rows_per_group + in_group;
-    if (in_group >= rows_per_group || row >= rows) return;
-    auto slot_of = [&](int c) { return (int64_t)2 * c + (c == c0 ? first : 0); };
-    float top = -INFINITY, sum = 0.0f;
-    bool dead = false;
-#pragma unroll 8
-    for (int c = c0; c <= c1; c++) {
-        const float2 x = ml[slot_of(c) * rows_per_group + in_group];
-        dead = dead || x.y < 0.0f;
-        top = fmaxf(top, x.x);
+    int n_active = 0;
+#pragma unroll
+    for (int i = 0; i < JOIN_RUNS; i++) {
+        const int c = 32 * i + lane;
+        const bool cut = c < TA_CTAS && cuts[c].parts > 0;
+        const uint32_t all = __ballot_sync(~0u, cut);
+        if (cut) active[warp][n_active + __popc(all & ((1u << lane) - 1))] = (int16_t)c;
+        n_active += __popc(all);
     }
-    if (top == -INFINITY) top = 0.0f;
-    const int quads = p.head_dim / 4, node = row / rep, head = kv * rep + row - node * rep;
-    for (int d = 4 * warp + lane % 4; d < quads; d += JOIN_THREADS / JOIN_ROWS) {
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        sum = 0.0f;
-#pragma unroll 8
-        for (int c = c0; c <= c1; c++) {
-            const int64_t slot = slot_of(c);
-            const float2 x = ml[slot * rows_per_group + in_group];
-            const float4 v = o[(slot * quads + d) * rows_per_group + in_group];
-            if (x.x == -INFINITY) continue;
-            const float f = exp2f(x.x - top);
-            sum += f * x.y;
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+    __syncwarp();
+    const int rep = p.n_head / p.n_kv_head, rows = p.n_node * rep, hd = p.head_dim;
+    const int groups = (rows + rows_per_group - 1) / rows_per_group;
+    const int per_warp = hd > 64 ? 1 : hd > 32 ? 2 : 4, wide = 32 / per_warp;  // rows to a warp, lanes to a row
+    const int runs = (min(rows, rows_per_group) + per_warp - 1) / per_warp;
+    const int64_t stride = part_stride(rows_per_group, hd);
+    float4 *mine = ahead + warp * JOIN_AHEAD * 32 + lane;
+    for (int w = blockIdx.x + gridDim.x * warp; w < n_active * runs; w += gridDim.x * JOIN_WARPS) {
+        const int who = active[warp][w / runs], first = w % runs * per_warp, c0 = who - 1;
+        const Cut cut = cuts[who];
+        const int parts = cut.parts, s = cut.s, kv = cut.item / groups, group = cut.item - kv * groups;
+        const int here = min(rows_per_group, rows - group * rows_per_group);  // rows of the group
+        auto slot_of = [&](int c) { return c ? 2 * (c0 + c) : cut.first_slot; };
+        const int r = lane / wide, in_group = first + r;
+        const bool real = in_group < here;
+        auto fetch = [&](int c, int d) {
+            if (c < parts && real && d < hd)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(mine + c % JOIN_AHEAD * 32)),
+                             "l"(o + slot_of(c) * stride + (int64_t)in_group * hd + d)
+                             : "memory");
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        };
+        const int row = group * rows_per_group + in_group, node = row / rep, head = kv * rep + row - node * rep;
+        T *out = (T *)p.out + s * p.out_seq + node * p.out_node + head * p.out_head;
+        if (parts <= JOIN_FEW) {
+            for (int d = 4 * (lane % wide); real && d < hd; d += 4 * wide) {
+                float2 x[JOIN_FEW];
+                float4 v[JOIN_FEW];
+                float top = -INFINITY, sum = 0.0f;
+                bool dead = false;
+#pragma unroll
+                for (int c = 0; c < JOIN_FEW; c++) {
+                    const int slot = slot_of(min(c, parts - 1));
+                    x[c] = ml[(int64_t)slot * rows_per_group + in_group];
+                    v[c] = *(const float4 *)(o + slot * stride + (int64_t)in_group * hd + d);
+                    if (c >= parts) x[c] = make_float2(-INFINITY, 0.0f);
+                }
+#pragma unroll
+                for (int c = 0; c < JOIN_FEW; c++) {
+                    dead = dead || x[c].y < 0.0f;
+                    top = fmaxf(top, x[c].x);
+                }
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < JOIN_FEW; c++) {
+                    const float f = x[c].x == -INFINITY ? 0.0f : exp2f(x[c].x - top);
+                    sum += f * x[c].y;
+                    if (f == 0.0f) v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    acc.x += f * v[c].x, acc.y += f * v[c].y, acc.z += f * v[c].z, acc.w += f * v[c].w;
+                }
+                store_quad(out + d, acc, dead || sum == 0.0f ? 0.0f : 1.0f / sum);
+            }
+            continue;
         }
-        const bool none = dead || sum == 0.0f;
-        const float inv = none ? 0.0f : 1.0f / sum;
-        T *out = (T *)p.out + s * p.out_seq + node * p.out_node + head * p.out_head + 4 * d;
-        struct alignas(4 * sizeof(T)) Quad { T v[4]; } q;
-        q.v[0] = from_f32<T>(none ? 0.0f : acc.x * inv), q.v[1] = from_f32<T>(none ? 0.0f : acc.y * inv);
-        q.v[2] = from_f32<T>(none ? 0.0f : acc.z * inv), q.v[3] = from_f32<T>(none ? 0.0f : acc.w * inv);
-        *(Quad *)out = q;
+        for (int c = 0; c < JOIN_AHEAD; c++) fetch(c, 4 * (lane % wide));
+        __syncwarp();  // the factors of the row before have been read
+        for (int k = 0; k < per_warp && first + k < here; k++) {
+            float2 x[JOIN_RUNS];
+            float top = -INFINITY, sum = 0.0f;
+            bool dead = false;
+#pragma unroll
+            for (int i = 0; i < JOIN_RUNS; i++) {
+                const int c = 32 * i + lane;
+                if (32 * i >= parts) break;
+                x[i] = c < parts ? ml[(int64_t)slot_of(c) * rows_per_group + first + k] : make_float2(-INFINITY, 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < JOIN_RUNS; i++) {
+                if (32 * i >= parts) break;
+                dead = dead || x[i].y < 0.0f;
+                top = fmaxf(top, x[i].x);
+            }
+            for (int b = 16; b; b >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, b));
+            dead = __any_sync(~0u, dead);
+#pragma unroll
+            for (int i = 0; i < JOIN_RUNS; i++) {
+                if (32 * i >= parts) break;
+                x[i].x = x[i].x == -INFINITY ? 0.0f : exp2f(x[i].x - top);
+                sum += x[i].x * x[i].y;
+            }
+            for (int b = 16; b; b >>= 1) sum += __shfl_xor_sync(~0u, sum, b);
+            const float inv = dead || sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < JOIN_RUNS; i++)
+                if (32 * i + lane < parts) factor[warp][k][32 * i + lane] = inv == 0.0f ? 0.0f : x[i].x * inv;
+        }
+        __syncwarp();
+        for (int d = 4 * (lane % wide); d < hd; d += 4 * wide) {
+            if (d >= 4 * wide)
+                for (int c = 0; c < JOIN_AHEAD; c++) fetch(c, d);
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int c = 0; c < parts; c++) {
+                asm volatile("cp.async.wait_group %0;\n" ::"n"(JOIN_AHEAD - 1) : "memory");
+                const float4 v = mine[c % JOIN_AHEAD * 32];  // (which this lane copied itself)
+                const float f = factor[warp][r][c];
+                fetch(c + JOIN_AHEAD, d);
+                if (f == 0.0f) continue;  // nothing seen there
+                acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+            }
+            if (real) store_quad(out + d, acc, 1.0f);
+        }
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     }
 }
 
@@ -197,11 +281,10 @@ void tree_launch(const sdy_tree_attention_args &a, cudaStream_t s) {
 
 }  // namespace
 
-void tree_join(const sdy_tree_attention_args &a, const TreeSpace &sp, int rows, int ctas, cudaStream_t s) {
-    const int total = a.n_node * (a.n_head / a.n_kv_head), groups = (total + rows - 1) / rows;
-    const dim3 grid((unsigned)(a.n_seq * a.n_kv_head * groups), (std::min(total, rows) + JOIN_ROWS - 1) / JOIN_ROWS);
+void tree_join(const sdy_tree_attention_args &a, const TreeSpace &sp, int rows, cudaStream_t s) {
     const auto kernel = a.type == T_F32 ? join_kernel<float> : a.type == T_F16 ? join_kernel<__half> : join_kernel<__nv_bfloat16>;
-    launch(kernel, grid, JOIN_THREADS, 0, s, a, (const int64_t *)sp.base, (const float4 *)sp.o, (const float2 *)sp.ml, rows, ctas);
+    launch(kernel, JOIN_BLOCKS, 32 * JOIN_WARPS, JOIN_WARPS * JOIN_AHEAD * 32 * sizeof(float4), s, a, (const Cut *)sp.cuts,
+           (const float *)sp.o, (const float2 *)sp.ml, rows);
     SDY_LAUNCHED();
 }
 

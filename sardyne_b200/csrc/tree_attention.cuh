@@ -10,27 +10,37 @@ constexpr int TA_MAX_NODES = 256;
 constexpr int TA_MAX_DIM = 256;
 
 // The split. A row group is the rows (node, query head) of one KV head of one sequence that a CTA
-// holds at once; a unit is one row group over one tile of keys. The units of a call, sequence by
-// sequence, KV head by KV head, row group by row group, tile by tile, are dealt to TA_CTAS CTAs in
-// equal contiguous shares (to as many CTAs as there are units, if fewer), whatever the lengths of the sequences, which only the device knows. A
-// CTA writes the result of a row group whose tiles it holds all; of one that its share cuts it
-// leaves the unnormalised sum, the maximum and the sum of weights in one of its two slots of the
-// workspace (first and last of its share), and join_kernel adds them up in the order of the CTAs.
+// holds at once. Its work is its tiles of keys and TA_SETUP more units for loading the queries and
+// storing the result (which for short sequences is most of the time). The units of a call, sequence
+// by sequence, KV head by KV head, row group by row group, are dealt to TA_CTAS CTAs in equal
+// contiguous shares, whatever the lengths of the sequences, which only the device knows. A CTA
+// writes the result of a row group whose tiles it holds all; of one that its share cuts it leaves
+// the unnormalised sum, the maximum and the sum of weights in one of its two slots of the workspace
+// (first and last row group of its share), and join_kernel adds them up in the order of the CTAs.
 constexpr int TA_CTAS = 148;  // one per SM
+constexpr int TA_SETUP = 3;
+
+// A row group to join, noted by the second CTA that holds tiles of it: the parts are the slot of
+// that CTA's predecessor and the first slots of the CTAs from it on.
+struct Cut {
+    int s, item, parts, first_slot;  // item: KV head x row groups + row group; parts 0: nothing to join
+};
 
 // Where things are in the workspace.
 struct TreeSpace {
-    int64_t *base;  // [n_seq + 1]: tiles of the sequences before
-    float *o;       // [TA_CTAS * 2][head_dim / 4][rows][4]
+    Cut *cuts;      // [TA_CTAS]
+    float *o;       // [TA_CTAS * 2] of part_stride floats: [rows][head_dim]
     float2 *ml;     // [TA_CTAS * 2][rows]: maximum (in log2 units), sum; sum < 0: padding
     size_t bytes;
 };
+// Floats from one slot to the next: off a power of two, so that a row's parts lie in all L2 slices.
+__host__ __device__ inline int64_t part_stride(int rows, int head_dim) { return (int64_t)rows * head_dim + 1088; }
 inline TreeSpace tree_space(const sdy_tree_attention_args &a, int rows) {
     TreeSpace t;
-    size_t at = align_up(((size_t)a.n_seq + 1) * 8, 256);
-    t.base = (int64_t *)a.ws;
+    size_t at = align_up(TA_CTAS * sizeof(Cut), 256);
+    t.cuts = (Cut *)a.ws;
     t.o = (float *)((uint8_t *)a.ws + at);
-    at += align_up((size_t)TA_CTAS * 2 * rows * a.head_dim * 4, 256);
+    at += align_up((size_t)TA_CTAS * 2 * part_stride(rows, a.head_dim) * 4, 256);
     t.ml = (float2 *)((uint8_t *)a.ws + at);
     t.bytes = at + align_up((size_t)TA_CTAS * 2 * rows * 8, 256);
     return t;
@@ -43,12 +53,15 @@ struct Lengths {
     int cached;  // of those, the ones that exist
     int keys;    // existing rows, drafted ones included (at least 1)
 };
-__device__ __forceinline__ Lengths lengths_of(const sdy_tree_attention_args &p, int s) {
+__device__ __forceinline__ Lengths lengths_of(const sdy_tree_attention_args &p, int s, int past) {
     Lengths l;
-    l.past = max(p.n_past[s], 0);
+    l.past = past;
     l.cached = min(l.past, p.max_seq);
     l.keys = (int)min((int64_t)l.past + p.n_node, (int64_t)p.max_seq);
     return l;
+}
+__device__ __forceinline__ Lengths lengths_of(const sdy_tree_attention_args &p, int s) {
+    return lengths_of(p, s, max(p.n_past[s], 0));
 }
 
 // Node above j: -1 for none, -2 when j is a padding node.
@@ -56,96 +69,133 @@ __device__ __forceinline__ int node_up(const int32_t *parent, int j) {
     const int up = parent ? parent[j] : j - 1;
     return up == -1 || (up >= 0 && up < j) ? up : -2;
 }
-// Does node j's path end in a root? Every step goes to an earlier node, so the walk ends.
-__device__ __forceinline__ bool node_live(const int32_t *parent, int j) {
-    while (j >= 0) j = node_up(parent, j);
+// The nodes above, checked, into shared memory by one warp; a walk along it calls at(node) from node
+// j on (negative: no walk) and is true for a path that ends in a root. Every step goes to an earlier
+// node, so walks end.
+__device__ __forceinline__ void load_tree(int16_t *up, const int32_t *parent, int n_node) {
+    for (int j = threadIdx.x % 32; j < n_node; j += 32) up[j] = (int16_t)node_up(parent, j);
+    __syncwarp();
+}
+template <class At> __device__ __forceinline__ bool walk_tree(const int16_t *up, int j, At at) {
+    while (j >= 0) {
+        at(j);
+        j = up[j];
+    }
     return j == -1;
 }
 
-// One CTA's share of the units, one run of tiles of one row group after the other.
+// First unit of CTA c's share, and the CTA whose share holds unit u. (Division by the constant.)
+__device__ __forceinline__ int64_t share_begin(int64_t units, int c) {
+    return units >= TA_CTAS ? units * c / TA_CTAS : min((int64_t)c, units);
+}
+__device__ __forceinline__ int share_of(int64_t units, int64_t u) {
+    return units >= TA_CTAS ? (int)(((u + 1) * TA_CTAS - 1) / units) : (int)u;
+}
+
+// One CTA's share, one run of tiles [t0, t1) of a row group after the other.
 struct Segment {
-    int s, head, group, t0, t1, tiles;  // tiles [t0, t1) of the group's `tiles`
+    int s, head, group, t0, t1, tiles, past;
 };
 template <int KEYS>
 struct Share {
     const sdy_tree_attention_args &p;
-    int64_t u, end, base;
-    int s, tiles, per_tile;  // per_tile: units per tile of a sequence
-    __device__ Share(const sdy_tree_attention_args &p_, int64_t u_, int64_t end_, int s_, int64_t base_, int per_tile_)
-        : p(p_), u(u_), end(end_), base(base_), s(s_), per_tile(per_tile_) {
-        tiles = u < end ? (lengths_of(p, s).keys + KEYS - 1) / KEYS : 0;
-    }
+    int64_t u, end, base;   // next unit, end, units of the sequences before s
+    int s, tiles, past, items;  // items: row groups per sequence
+    __device__ Share(const sdy_tree_attention_args &p_, const int64_t *found, int items_)
+        : p(p_), u(found[0]), end(found[1]), base(found[3]), s((int)found[2]), tiles((int)found[4]),
+          past((int)found[6]), items(items_) {}
+    // The next run; runs that hold no tile (only the end of a row group's setup) are passed over.
     __device__ bool next(Segment &g, int groups) {
-        if (u >= end) return false;
-        while (u >= (base + tiles) * per_tile) {
-            base += tiles;
-            tiles = (lengths_of(p, ++s).keys + KEYS - 1) / KEYS;
+        while (u < end) {
+            while (u >= base + (int64_t)(tiles + TA_SETUP) * items) {
+                base += (int64_t)(tiles + TA_SETUP) * items;
+                s++;
+                past = max(p.n_past[s], 0);
+                tiles = (lengths_of(p, s, past).keys + KEYS - 1) / KEYS;
+            }
+            const int64_t r = u - base;
+            const int per = tiles + TA_SETUP, item = r >> 31 ? (int)(r / per) : (int)((unsigned)r / (unsigned)per);
+            const int at = (int)(r - (int64_t)item * per);
+            const int to = (int)min((int64_t)per, at + end - u);
+            u += to - at;
+            if (to <= TA_SETUP) continue;
+            g.s = s;
+            g.head = item / groups;
+            g.group = item - g.head * groups;
+            g.tiles = tiles;
+            g.past = past;
+            g.t0 = max(at - TA_SETUP, 0);
+            g.t1 = to - TA_SETUP;
+            return true;
         }
-        const int64_t r = u - base * per_tile;
-        const int item = (int)(r / tiles);
-        g.s = s;
-        g.head = item / groups;
-        g.group = item - g.head * groups;
-        g.tiles = tiles;
-        g.t0 = (int)(r - (int64_t)item * tiles);
-        g.t1 = (int)min((int64_t)tiles, g.t0 + end - u);
-        u += g.t1 - g.t0;
-        return true;
+        return false;
     }
 };
 
 // Where CTA `cta`'s share begins, found by the whole block (THREADS threads, all of them): the
-// tiles before each run of sequences by a scan over the threads, the rest by walking that run.
-// out[0..3] = first unit, end, first sequence, tiles before it. CTA 0 also leaves the table of
-// tiles before every sequence for join_kernel.
+// units before each run of sequences by a scan over the threads, the rest by walking that run.
+// out[0..6] = first unit, end, first sequence, units before it, its tiles, all units, its length.
 template <int KEYS, int THREADS>
-__device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int per_tile, int cta, int ctas,
-                                           int64_t *base_table, int64_t *scan /* THREADS + 1 */, int64_t *out) {
+__device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int items, int cta,
+                                           int64_t *scan /* THREADS / 32 */, int64_t *out) {
     const int t = threadIdx.x, run = (p.n_seq + THREADS - 1) / THREADS;
     const int s0 = min(t * run, p.n_seq), s1 = min(s0 + run, p.n_seq);
+    auto tiles_of = [&](int s) { return (lengths_of(p, s).keys + KEYS - 1) / KEYS; };
     int64_t mine = 0;
-    for (int s = s0; s < s1; s++) mine += (lengths_of(p, s).keys + KEYS - 1) / KEYS;
+    for (int s = s0; s < s1; s++) mine += tiles_of(s) + TA_SETUP;
     int64_t sum = mine;  // inclusive over the warp
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t v = __shfl_up_sync(~0u, sum, o);
         if (t % 32 >= o) sum += v;
     }
     if (t % 32 == 31) scan[t / 32] = sum;
+    if (t == 0) out[2] = out[3] = out[4] = out[6] = 0;
     __syncthreads();
     int64_t before = 0, total = 0;
+#pragma unroll
     for (int w = 0; w < THREADS / 32; w++) {
         if (w < t / 32) before += scan[w];
         total += scan[w];
     }
     before += sum - mine;
-    const int64_t units = total * per_tile, n = min((int64_t)ctas, units);
-    const int64_t u0 = cta < n ? units * cta / n : 0, u1 = cta < n ? units * (cta + 1) / n : 0;
-    if (t == 0) out[0] = u0, out[1] = u1, out[2] = 0, out[3] = 0;
-    __syncthreads();
-    if (u0 < u1 && u0 >= before * per_tile && u0 < (before + mine) * per_tile) {
-        int s = s0;
-        for (int64_t b = before;; s++) {
-            const int64_t n = (lengths_of(p, s).keys + KEYS - 1) / KEYS;
-            if (u0 < (b + n) * per_tile) {
-                out[2] = s, out[3] = b;
-                break;
-            }
-            b += n;
+    const int64_t units = total * items;
+    const int64_t u0 = share_begin(units, cta), u1 = share_begin(units, cta + 1);
+    if (t == 0) out[0] = u0, out[1] = u1, out[5] = units;
+    if (u0 < u1 && u0 >= before * items && u0 < (before + mine) * items) {
+        int s = s0, n = run == 1 ? (int)mine - TA_SETUP : tiles_of(s0);
+        int64_t b = before * items;
+        while (u0 >= b + (int64_t)(n + TA_SETUP) * items) {
+            b += (int64_t)(n + TA_SETUP) * items;
+            s++;
+            n = tiles_of(s);
         }
-    }
-    if (cta == 0) {
-        for (int s = s0; s < s1; s++) {
-            base_table[s] = before;
-            before += (lengths_of(p, s).keys + KEYS - 1) / KEYS;
-        }
-        if (t == 0) base_table[p.n_seq] = total;
+        out[2] = s, out[3] = b, out[4] = n, out[6] = max(p.n_past[s], 0);
     }
     __syncthreads();
+}
+// What CTA `cta` notes for join_kernel (one thread, after find_share).
+template <int KEYS>
+__device__ __forceinline__ void note_cut(const sdy_tree_attention_args &p, int items, int groups, int cta, const int64_t *found,
+                                         Cut *cuts) {
+    Cut cut = {0, 0, 0, 0};
+    Share<KEYS> share(p, found, items);
+    Segment g;
+    if (share.next(g, groups) && g.t0 > 0) {
+        const int64_t units = found[5], item = g.head * groups + g.group;
+        const int64_t u0 = share.base + item * (g.tiles + TA_SETUP);
+        const int first = share_of(units, u0 + TA_SETUP);  // the CTA that holds the first tile
+        if (first == cta - 1) {
+            cut.s = g.s, cut.item = (int)item;
+            cut.parts = share_of(units, u0 + TA_SETUP + g.tiles - 1) - first + 1;
+            cut.first_slot = 2 * first + (share_begin(units, first) < u0);
+        }
+    }
+    cuts[cta] = cut;
 }
 #endif
 
 // out of the partial results (tree_attention.cu). rows: rows per group.
-void tree_join(const sdy_tree_attention_args &a, const TreeSpace &sp, int rows, int ctas, cudaStream_t s);
+void tree_join(const sdy_tree_attention_args &a, const TreeSpace &sp, int rows, cudaStream_t s);
 
 // 16-bit caches of up to 128 elements a head on the tensor cores (tree_attention_tc.cu).
 bool tree_tc_takes(const sdy_tree_attention_args &a);

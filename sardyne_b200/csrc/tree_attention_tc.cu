@@ -1,20 +1,23 @@
 // Tree attention over 16-bit caches on the tensor cores (tcgen05, accumulators in TMEM).
 //
 // For one KV head of one sequence the rows are its (node, query head) pairs, 128 to an MMA tile;
-// per tile of 128 keys, S = Q K^T (128 x 128, f32 in TMEM), P = 2^(c S - m) as 16-bit values over
-// S's own columns, O += P V with P read from TMEM. m is a row's running maximum; O and the sum are
-// rescaled only when it has grown by more than 2^8 since it was last set (the division by the sum
-// takes out any common factor; 2^8 keeps P inside the range of f16), which after the first tiles
-// hardly ever happens, so O stays in TMEM.
+// per tile of 80 keys, S = Q K^T (128 x 80, f32 in TMEM), P = 2^(c S - m) as 16-bit values in TMEM,
+// O += P V with P as the A operand. m is a row's running maximum; O and the sum are rescaled only
+// when it has grown by more than 2^8 since it was last set (the division by the sum takes out any
+// common factor; 2^8 keeps P inside the range of f16), which after the first tiles hardly ever
+// happens, so O stays in TMEM.
 //
-// One CTA per SM, twelve warps: a TMA producer (K and V tiles of 128 keys through a ring of shared
-// memory slots), an MMA issuer, and two streams of four warps that turn S into P, one row to a
-// thread, so that one stream's exponentials run under the other's MMAs. With more than 128 rows the
-// streams hold two row tiles and share every K and V tile (DUAL); with fewer they share the rows
-// and take the tiles in turn, and the first stream joins the two results at the end.
+// One CTA per SM, twelve warps: a TMA producer (K and V tiles through a ring of shared memory
+// slots), an MMA issuer, and two streams of four warps that turn S into P, one row to a thread. With
+// more than 128 rows the streams hold two row tiles and share every K and V tile (DUAL); with fewer
+// they share the rows and take the tiles in turn, and the first stream joins the two results at the
+// end. 80 keys: S and P then fit side by side beside O in a stream's half of TMEM (80 + 40 of 128
+// columns), so the next S is formed while the exponentials of this one run; with tiles of 128 keys and
+// P over S's own columns each stream waited for P V and the next Q K^T in turn, 3400 cycles per 2 x 128
+// rows and 128 keys (measured on B200, 2 x 64 nodes, 32 heads, 65537 keys).
 //
-// Bound by the tensor pipe and the exponentials alike from about 256 rows (128 x 128 scores take
-// 1024 cycles of MMA and 1024 of the exponential unit), by HBM below about 64.
+// Bound by the exponentials (16 a cycle) and the shared memory reads of Q K^T alike from about 256
+// rows, by HBM below about 64.
 #include "tree_attention.cuh"
 
 #include <cuda.h>
@@ -30,23 +33,26 @@ namespace {
 constexpr int TK = 128;       // keys per tile
 constexpr int TR = 128;       // rows per MMA tile
 constexpr int TT = 384;       // threads
-constexpr int CHUNK = TK * 128;  // bytes of 64 elements of 128 rows, 128-byte swizzled
-constexpr long long WAIT_LIMIT = 1ll << 22;  // mbarrier polls before giving up (about a second)
-constexpr uint32_t TM_S = 0, TM_O = 256;     // TMEM columns of the streams' S and O, 128 each
+constexpr int CHUNK = TK * 128, QCHUNK = TR * 128;  // bytes of 64 elements of a tile's rows, 128-byte swizzled
+constexpr int WAIT_LIMIT = 1 << 22;  // mbarrier polls before giving up (about a second)
+constexpr uint32_t TM_S = 0, TM_O = 256;     // TMEM columns of stream 0's S (and P over it) and O; stream 1's are 128 on
 constexpr float GROWTH = 8.0f;
 
 __device__ unsigned g_tree_status;  // nonzero: a wait ran out
 
-constexpr int tc_slots(bool dual, int hc) { return hc == 1 ? 10 : dual ? 5 : 6; }
-constexpr int tc_smem(bool dual, int hc) { return ((dual ? 2 : 1) + tc_slots(dual, hc)) * hc * CHUNK + 1024; }
+constexpr int SLOTS = 12;  // ring slots, at most
+// Slots of a ring: one ring for both streams (DUAL), or one for each.
+constexpr int tc_slots(bool dual, int hc) { return dual ? 10 / hc : 6 / hc; }
+constexpr int tc_smem(bool dual, int hc) { return (dual ? 2 : 1) * hc * QCHUNK + (dual ? 1 : 2) * tc_slots(dual, hc) * hc * CHUNK; }
 
 struct Shared {
-    uint64_t full[10], empty[10];
+    uint64_t full[SLOTS], empty[SLOTS];
     uint64_t q_ready[2], s_full[2], p_ready[2], o_done[2];
-    uint64_t merge_full, merge_done, drain;
-    uint32_t tmem, abort;
+    uint64_t merge_full, merge_done, drain[2];
+    uint32_t tmem;
     int odd;  // the last segment (from 1) whose drafted V rows hold NaN or infinities
-    int64_t scan[TT / 32], share[4];
+    int64_t scan[TT / 32], share[7];
+    int16_t up[2][TA_MAX_NODES];  // per stream (its warps are in one segment while they walk)
     float2 ml[TR];
 };
 
@@ -60,27 +66,26 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *b) {
 __device__ __forceinline__ void mbar_expect(uint64_t *b, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
 }
-// Bounded: false, with the abort flag set, when the limit ran out here or in another role.
-__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity, Shared *sh) {
-    const uint32_t bar = smem_u32(b);
-    for (long long it = 0; it < WAIT_LIMIT; it++) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-        if ((it & 255) == 255 && *(volatile uint32_t *)&sh->abort) return false;
-    }
-    *(volatile uint32_t *)&sh->abort = 1;
-    return false;
+// Bounded: false when the limit ran out. A few instructions only: the code of the roles shares the
+// instruction caches, and the MMA issuer's waits are on the critical path.
+__device__ __forceinline__ bool mbar_wait(uint64_t *b, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 n;\n\tmov.u32 n, %3;\n"
+        "again:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "@p bra done;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "setp.ne.u32 p, n, 0;\n\t"
+        "@p bra again;\n"
+        "done:\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(b)), "r"(parity), "n"(WAIT_LIMIT)
+        : "memory");
+    return ok != 0;
 }
-__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, Shared *sh) {
-    return __all_sync(~0u, mbar_wait(b, parity, sh));
-}
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity) { return __all_sync(~0u, mbar_wait(b, parity)); }
 
 __device__ __forceinline__ void tma_tile(const CUtensorMap *map, uint64_t *bar, uint32_t dst, int x, int row, int head, int s) {
     asm volatile(
@@ -91,25 +96,30 @@ __device__ __forceinline__ void tma_tile(const CUtensorMap *map, uint64_t *bar, 
 
 // Shared memory descriptors of tiles in the 128-byte swizzle: K-major (Q and K: 8-row groups of
 // 1024 bytes) and N-major (V: 64-element chunks at CHUNK, 8-key groups of 1024 bytes).
-__device__ __forceinline__ uint64_t desc_of(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// The low word holds the address and LBO, the high word SBO, the version and the swizzle.
+constexpr uint32_t DESC_HI = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | (lbo >> 4) << 16; }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one != 0;
 }
 // kind::f16: f32 accumulator, A and B of one 16-bit type, M = 128; b_mn: B is N-major.
 __device__ __forceinline__ uint32_t idesc_f16(bool bf16, int n, bool b_mn) {
     return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_mn ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(TR >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI)
         : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t *b) {
@@ -119,10 +129,6 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 
-#define R32(v, o)                                                                                                       \
-    v[o], v[o + 1], v[o + 2], v[o + 3], v[o + 4], v[o + 5], v[o + 6], v[o + 7], v[o + 8], v[o + 9], v[o + 10], v[o + 11], \
-        v[o + 12], v[o + 13], v[o + 14], v[o + 15], v[o + 16], v[o + 17], v[o + 18], v[o + 19], v[o + 20], v[o + 21],     \
-        v[o + 22], v[o + 23], v[o + 24], v[o + 25], v[o + 26], v[o + 27], v[o + 28], v[o + 29], v[o + 30], v[o + 31]
 #define OUT4(v, o) "=f"(v[o]), "=f"(v[o + 1]), "=f"(v[o + 2]), "=f"(v[o + 3])
 #define IN4(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3])
 #define LIST32                                                                                                        \
@@ -134,9 +140,15 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, float *v) {
                  : OUT4(v, 0), OUT4(v, 4), OUT4(v, 8), OUT4(v, 12), OUT4(v, 16), OUT4(v, 20), OUT4(v, 24), OUT4(v, 28)
                  : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t *v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " LIST32 ";\n" ::IN4(v, 0), IN4(v, 4), IN4(v, 8), IN4(v, 12),
-                 IN4(v, 16), IN4(v, 20), IN4(v, 24), IN4(v, 28), "r"(addr)
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float *v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+                 "[%16];\n"
+                 : OUT4(v, 0), OUT4(v, 4), OUT4(v, 8), OUT4(v, 12)
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                 "%14, %15};\n" ::IN4(v, 0), IN4(v, 4), IN4(v, 8), IN4(v, 12), "r"(addr)
                  : "memory");
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
@@ -156,165 +168,203 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *(uint32_t *)&h;
 }
-// Of two packed 16-bit values, the ones that are NaN or infinite replaced by zero.
+// Nonzero when one of two packed 16-bit values is NaN or infinite (an exponent of ones: adding one
+// to it carries into the sign's place), and the pair with such values replaced by zero.
+template <class T> __device__ __forceinline__ uint32_t infinite2(uint32_t w) {
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7C007C00u : 0x7F807F80u, ONE = E & ~(E << 1);
+    return ((w & E) + ONE) & 0x80008000u;
+}
 template <class T> __device__ __forceinline__ uint32_t finite2(uint32_t w) {
-    constexpr uint32_t E = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-    if ((w & E) == E) w &= 0xFFFF0000u;
-    if (((w >> 16) & E) == E) w &= 0x0000FFFFu;
-    return w;
+    const uint32_t bad = infinite2<T>(w);
+    return w & ~((bad & 0x8000u ? 0xFFFFu : 0u) | (bad & 0x80000000u ? 0xFFFF0000u : 0u));
 }
 
-// Position in the ring's load order, counted from the segment's first load, of tile i's K and V:
-// the order in which the MMAs take them.
-template <bool DUAL> __device__ __forceinline__ int k_pos(int i) { return DUAL ? 2 * i : i < 2 ? i : 2 * i - 1; }
-template <bool DUAL> __device__ __forceinline__ int v_pos(int i, int n) {
-    return DUAL || i == n - 1 ? 2 * i + 1 : 2 * i + 2;
+// The paths of up to 64 nodes by pointer doubling over the warp, which holds the nodes above lane and
+// lane + 32 in up[]: after k rounds a node knows 2^k nodes of its way. `path` is that of `node`,
+// `alive` has the nodes whose way ends in a root.
+__device__ __forceinline__ void warp_paths(const int (&above)[2], int n_node, int node, uint64_t &path, uint64_t &alive) {
+    const int lane = threadIdx.x % 32;
+    int up[2] = {above[0], above[1]};
+    uint64_t bits[2] = {1ull << lane, 1ull << (lane + 32)};
+    const bool wide = n_node > 32;
+    for (int hop = 1; hop < n_node; hop *= 2) {
+        int to[2];
+        uint64_t more[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            to[w] = -2, more[w] = 0;
+            if (w && !wide) continue;
+            const int from = up[w] & 31;
+            const int t0 = __shfl_sync(~0u, up[0], from);
+            const uint64_t b0 = __shfl_sync(~0u, bits[0], from);
+            to[w] = t0, more[w] = b0;
+            if (wide) {
+                const int t1 = __shfl_sync(~0u, up[1], from);
+                const uint64_t b1 = __shfl_sync(~0u, bits[1], from);
+                if (up[w] >= 32) to[w] = t1, more[w] = b1;
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+            if (up[w] >= 0) {
+                bits[w] |= more[w];
+                up[w] = to[w];
+            }
+    }
+    const uint64_t p0 = __shfl_sync(~0u, bits[0], node & 31), p1 = __shfl_sync(~0u, bits[1], node & 31);
+    path = node < 32 ? p0 : p1;
+    alive = __ballot_sync(~0u, up[0] == -1) | (uint64_t)__ballot_sync(~0u, wide && up[1] == -1) << 32;
 }
 
 template <class T, bool DUAL, int HC>
 __global__ void __launch_bounds__(TT, 1)
     tree_tc_kernel(const sdy_tree_attention_args p, const __grid_constant__ CUtensorMap kmap,
-                   const __grid_constant__ CUtensorMap vmap, int64_t *base_table, float *part_o, float2 *part_ml) {
-    constexpr int NS = tc_slots(DUAL, HC), NQ = DUAL ? 2 : 1, LEAD = DUAL ? 1 : 2;
-    constexpr int TILE = HC * CHUNK, ROWS = NQ * TR;
+                   const __grid_constant__ CUtensorMap vmap, Cut *cuts, float *part_o, float2 *part_ml) {
+    constexpr int NQ = DUAL ? 2 : 1, STEP = DUAL ? 1 : 2;  // a stream takes every STEP-th tile
+    constexpr int NS = tc_slots(DUAL, HC);                  // slots of a ring: K, V, K, V, .. of its tiles
+    constexpr int TILE = HC * CHUNK, QTILE = HC * QCHUNK, ROWS = NQ * TR;
     constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
     __shared__ Shared sh;
-    extern __shared__ uint8_t dyn[];
-    uint8_t *qbuf = (uint8_t *)(((uintptr_t)dyn + 1023) & ~(uintptr_t)1023), *ring = qbuf + NQ * TILE;
+    extern __shared__ __align__(1024) uint8_t qbuf[];
+    uint8_t *ring = qbuf + NQ * QTILE;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rep = p.n_head / p.n_kv_head, rows = p.n_node * rep, groups = (rows + ROWS - 1) / ROWS;
     const int n_pv = (p.head_dim + 15) & ~15, k_steps = (p.head_dim + 15) / 16;
 
+    if (warp == 3 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(&vmap) : "memory");
+    }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&sh.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
+        for (int i = 0; i < NS * STEP; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], NQ);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.q_ready[i], TR), mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_ready[i], TR), mbar_init(&sh.o_done[i], 1);
         }
-        mbar_init(&sh.merge_full, TR), mbar_init(&sh.merge_done, TR), mbar_init(&sh.drain, 1);
+        mbar_init(&sh.merge_full, TR), mbar_init(&sh.merge_done, TR), mbar_init(&sh.drain[0], 1), mbar_init(&sh.drain[1], 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        sh.abort = 0, sh.odd = 0;
+        sh.odd = 0;
     }
     pdl_wait();
-    find_share<TK, TT>(p, p.n_kv_head * groups, blockIdx.x, gridDim.x, base_table, sh.scan, sh.share);
+    find_share<TK, TT>(p, p.n_kv_head * groups, blockIdx.x, sh.scan, sh.share);
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = sh.tmem;
-    Share<TK> share(p, sh.share[0], sh.share[1], (int)sh.share[2], sh.share[3], p.n_kv_head * groups);
+    Share<TK> share(p, sh.share, p.n_kv_head * groups);
     Segment g;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            int pos = 0;  // loads so far
+    // registers go to the two warpgroups that hold rows: 96 x 128 + 200 x 256 <= 168 x 384
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n" ::);
+        if (warp == 0 && lane == 0) {
+            int pos[STEP] = {};  // loads so far, per ring
             bool ok = true;
-            auto load = [&](const CUtensorMap *map, int tile) {
-                const int slot = pos % NS, turn = pos / NS;
-                if (turn && !mbar_wait(&sh.empty[slot], (turn - 1) & 1, &sh)) return false;
+            auto load = [&](const CUtensorMap *map, int r, int i) {  // the stream's tile i into ring r
+                const int slot = r * NS + pos[r] % NS, turn = pos[r] / NS;
+                if (turn && !mbar_wait(&sh.empty[slot], (turn - 1) & 1)) return false;
+                // the first queries do not queue behind rings full of tiles
+                if (r == 0 && pos[0] == 1 && !(mbar_wait(&sh.q_ready[0], 0) && (!DUAL || mbar_wait(&sh.q_ready[1], 0)))) return false;
                 mbar_expect(&sh.full[slot], TILE);
                 for (int c = 0; c < HC; c++)
-                    tma_tile(map, &sh.full[slot], smem_u32(ring + slot * TILE + c * CHUNK), 64 * c, tile * TK, g.head, g.s);
-                pos++;
+                    tma_tile(map, &sh.full[slot], smem_u32(ring + slot * TILE + c * CHUNK), 64 * c, (g.t0 + i * STEP + r) * TK, g.head, g.s);
+                pos[r]++;
                 return true;
             };
             while (ok && share.next(g, groups)) {
                 const int n = g.t1 - g.t0;
-                for (int i = 0; ok && i < min(LEAD, n); i++) ok = load(&kmap, g.t0 + i);
-                for (int i = 0; ok && i < n; i++) {
-                    ok = load(&vmap, g.t0 + i);
-                    if (ok && i + LEAD < n) ok = load(&kmap, g.t0 + i + LEAD);
+                for (int i = 0; ok && i < n; i += STEP) {
+#pragma unroll
+                    for (int r = 0; r < STEP; r++)
+                        if (i + r < n) ok = ok && load(&kmap, r, i / STEP) && load(&vmap, r, i / STEP);
                 }
             }
             if (!ok) {  // let the copies in flight land before the memory is given up
-                sh.abort = 1;
                 atomicOr(&g_tree_status, 1u);
-                for (int q = max(0, pos - NS); q < pos; q++)
-                    for (long long it = 0; it < WAIT_LIMIT; it++) {
-                        uint32_t done;
-                        asm volatile(
-                            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-                            : "=r"(done)
-                            : "r"(smem_u32(&sh.full[q % NS])), "r"(q / NS & 1)
-                            : "memory");
-                        if (done) break;
-                    }
+                for (int r = 0; r < STEP; r++)
+                    for (int q = max(0, pos[r] - NS); q < pos[r]; q++) mbar_wait(&sh.full[r * NS + q % NS], q / NS & 1);
             }
         }
-        __syncwarp();
-    } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t id_qk = idesc_f16(BF, TK, false), id_pv = idesc_f16(BF, n_pv, true);
-            int base = 0, seg = 0;        // ring position of the segment's first load, segments so far
-            uint32_t p_parity[2] = {0, 0};
-            bool ok = true;
-            auto wait_full = [&](int pos) { return mbar_wait(&sh.full[pos % NS], pos / NS & 1, &sh); };
-            auto qk = [&](int st, int pos) {
-                const uint32_t qa = smem_u32(qbuf + (DUAL ? st : 0) * TILE), ka = smem_u32(ring + pos % NS * TILE);
-                for (int k = 0; k < k_steps; k++) {
-                    const uint32_t off = (k / 4) * CHUNK + (k % 4) * 32;
-                    mma_ss(tmem + TM_S + st * 128, desc_of(qa + off, 16, 1024), desc_of(ka + off, 16, 1024), id_qk, k > 0);
+        if (warp == 3 && lane == 0) note_cut<TK>(p, p.n_kv_head * groups, groups, blockIdx.x, sh.share, cuts);
+        if (warp == 3) {  // the queries of the share into L2, ahead of the loads that keep HBM busy
+            while (share.next(g, groups)) {
+                const int first = g.group * ROWS, last = min(rows, first + ROWS);
+                for (int r = first + lane; r < last; r += 32) {
+                    const int node = r / rep;
+                    const T *q = (const T *)p.q + g.s * p.q_seq + node * p.q_node + (g.head * rep + r - node * rep) * p.q_head;
+                    for (int e = 0; e < p.head_dim; e += 64) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q + e));
                 }
-                mma_commit(&sh.s_full[st]);
+            }
+        }
+        if (warp == 1 || warp == 2) {
+            // A warp issues for one stream: a wait on a barrier that is complete takes 100 cycles and the
+            // tensor pipe queues little, so with one warp for both it would idle during every wait. The
+            // whole warp waits, one lane issues; the shuffles tell the compiler that the operands are the
+            // same in all lanes (the tensor instructions take them from uniform registers).
+            auto uniform = [](uint32_t x) { return __shfl_sync(~0u, x, 0); };
+            const int st = (int)uniform(warp - 1), first_slot = DUAL ? 0 : st * NS;
+            const uint32_t id_qk = uniform(idesc_f16(BF, TK, false)), id_pv = uniform(idesc_f16(BF, n_pv, true));
+            const uint32_t q_lo = uniform(desc_lo(smem_u32(qbuf + (DUAL ? st : 0) * QTILE), 16)), steps = uniform(k_steps);
+            const uint32_t k_lo = uniform(desc_lo(smem_u32(ring), 16)), v_lo = uniform(desc_lo(smem_u32(ring), CHUNK));
+            const uint32_t tm_s = uniform(tmem) + TM_S + st * 128, tm_o = tm_s - TM_S + TM_O;
+            int base = 0, seg = 0;  // ring position of the segment's first load, segments so far
+            uint32_t p_parity = 0;
+            bool ok = true;
+            auto slot_of = [&](int pos) { return first_slot + pos % NS; };
+            auto wait_full = [&](int pos) { return warp_wait(&sh.full[slot_of(pos)], pos / NS & 1); };
+            auto qk = [&](int pos) {
+                const uint32_t b = uniform(k_lo + slot_of(pos) * (TILE >> 4));
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < 4 * HC; k++)
+                        if (k < steps)
+                            mma_ss(tm_s, q_lo + (((k / 4) * QCHUNK + (k % 4) * 32) >> 4), b + (((k / 4) * CHUNK + (k % 4) * 32) >> 4), id_qk, k > 0);
+                    mma_commit(&sh.s_full[st]);
+                    mma_commit(&sh.empty[slot_of(pos)]);
+                }
             };
-            auto pv = [&](int st, int pos, bool first) {
-                const uint32_t va = smem_u32(ring + pos % NS * TILE);
-                for (int k = 0; k < TK / 16; k++)
-                    mma_ts(tmem + TM_O + st * 128, tmem + TM_S + st * 128 + 8 * k, desc_of(va + 2048 * k, CHUNK, 1024), id_pv,
-                           k > 0 || !first);
+            auto pv = [&](int pos, bool first) {
+                const uint32_t b = uniform(v_lo + slot_of(pos) * (TILE >> 4)), again = uniform(!first);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < TK / 16; k++) mma_ts(tm_o, tm_s + 8 * k, b + (2048 * k >> 4), id_pv, k > 0 ? 1u : again);
+                    mma_commit(&sh.empty[slot_of(pos)]);
+                }
             };
             while (ok && share.next(g, groups)) {
-                const int n = g.t1 - g.t0;
-                for (int st = 0; ok && st < NQ; st++) ok = mbar_wait(&sh.q_ready[st], seg & 1, &sh);
-                for (int i = 0; ok && i < min(LEAD, n); i++) {
-                    const int pos = base + k_pos<DUAL>(i);
-                    if (!(ok = wait_full(pos))) break;
-                    fence_after();
-                    for (int st = DUAL ? 0 : i; st < (DUAL ? 2 : i + 1); st++) qk(st, pos);
-                    mma_commit(&sh.empty[pos % NS]);
+                const int n = (g.t1 - g.t0 + STEP - 1 - (DUAL ? 0 : st)) / STEP;  // the stream's tiles
+                if (!(ok = warp_wait(&sh.q_ready[DUAL ? st : 0], seg & 1))) break;
+                fence_after();
+                if (n) {
+                    if (!(ok = wait_full(base))) break;
+                    qk(base);
                 }
-                for (int i = 0; ok && i < n; i++) {
-                    const int vp = base + v_pos<DUAL>(i, n), kp = base + k_pos<DUAL>(i + LEAD);
-                    const bool more = i + LEAD < n;
-                    for (int st = DUAL ? 0 : i & 1; ok && st < (DUAL ? 2 : (i & 1) + 1); st++) {
-                        if (!(ok = mbar_wait(&sh.p_ready[st], p_parity[st], &sh))) break;
-                        p_parity[st] ^= 1;
-                        if (!(ok = wait_full(vp))) break;
-                        fence_after();
-                        pv(st, vp, DUAL ? i == 0 : i < 2);
-                        if (!DUAL || st == 1) mma_commit(&sh.empty[vp % NS]);
-                        if (more) {
-                            if (!(ok = wait_full(kp))) break;
-                            qk(st, kp);
-                            if (!DUAL || st == 1) mma_commit(&sh.empty[kp % NS]);
-                        } else {
-                            mma_commit(&sh.o_done[st]);
-                        }
-                    }
+                for (int i = 0; i < n; i++) {
+                    const int pos = base + 2 * i + 1;
+                    // both tiles are waited for first: P is what comes last
+                    if (!(ok = wait_full(pos) && (i + 1 == n || wait_full(pos + 1)) && warp_wait(&sh.p_ready[st], p_parity))) break;
+                    p_parity ^= 1;
+                    fence_after();
+                    pv(pos, i == 0);
+                    if (i + 1 < n) qk(pos + 1);  // over P, which the MMAs before have read by then
+                    else if (elect_one()) mma_commit(&sh.o_done[st]);
                 }
                 base += 2 * n;
                 seg++;
             }
             if (!ok) {  // the MMAs in flight end before the tensor memory is freed
-                atomicOr(&g_tree_status, 1u);
-                sh.abort = 1;
-                mma_commit(&sh.drain);
-                for (long long it = 0; it < WAIT_LIMIT; it++) {
-                    uint32_t done;
-                    asm volatile(
-                        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], 0;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-                        : "=r"(done)
-                        : "r"(smem_u32(&sh.drain))
-                        : "memory");
-                    if (done) break;
-                }
+                if (lane == 0) atomicOr(&g_tree_status, 1u);
+                if (elect_one()) mma_commit(&sh.drain[st]);
+                warp_wait(&sh.drain[st], 0);
             }
         }
         __syncwarp();
-    } else if (warp >= 4) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n" ::);
         const int st = (warp - 4) / 4, tid = threadIdx.x - 128 - 128 * st;  // stream, row of its tile
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;                  // 32 lanes to a warp
         const uint32_t tm_s = tmem + TM_S + st * 128 + lanes, tm_o = tmem + TM_O + st * 128 + lanes;
@@ -325,73 +375,123 @@ __global__ void __launch_bounds__(TT, 1)
         uint32_t s_parity = 0, o_parity = 0;
         bool ok = true;
         while (ok && share.next(g, groups)) {
-            const int n = g.t1 - g.t0;
-            const Lengths len = lengths_of(p, g.s);
+            const int n = (g.t1 - g.t0 + STEP - 1 - (DUAL ? 0 : st)) / STEP;  // the stream's tiles
+            const Lengths len = lengths_of(p, g.s, g.past);
             const int32_t *parent = p.parent ? p.parent + (int64_t)g.s * p.n_node : nullptr;
             const int row = g.group * ROWS + (DUAL ? st * TR : 0) + tid;
             const bool real = row < rows;
             const int node = real ? row / rep : 0, head = g.head * rep + (real ? row - node * rep : 0);
             const bool busy = __any_sync(~0u, real);  // a warp without rows does no arithmetic
-            if (DUAL || st == 0) {  // this row of Q into the swizzled tile
-                const T *q = (const T *)p.q + g.s * p.q_seq + node * p.q_node + head * p.q_head;
-                uint8_t *dst = qbuf + (DUAL ? st : 0) * TILE + tid * 128;
+            const bool edges = g.t1 * TK > len.cached;  // drafted rows, or none at all, in the last tiles
+            int parent_of[2] = {-2, -2};                // of nodes lane and lane + 32
+            if (edges && p.n_node <= 64)
+                for (int w = 0; w < 2; w++)
+                    if (lane + 32 * w < p.n_node) parent_of[w] = node_up(parent, lane + 32 * w);
+            const int64_t q_at = g.s * p.q_seq + node * p.q_node + head * p.q_head;
+            if (DUAL || st == 0) {  // the warp's rows of Q into the swizzled tile, a run of lanes to a row
+                constexpr int PER = HC * 8;  // lanes to a row: 16 bytes each
+                uint8_t *dst = qbuf + (DUAL ? st : 0) * QTILE + (warp % 4) * 32 * 128;
+                const int j = lane % PER, rows_left = rows - (row - lane);
+                uint4 v[PER];
 #pragma unroll
-                for (int j = 0; j < HC * 8; j++) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (real && j < chunks) v = *(const uint4 *)(q + 8 * j);
-                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                    *(uint4 *)(dst + (j / 8) * CHUNK + (((j & 7) ^ (tid & 7)) << 4)) = v;
+                for (int i = 0; i < PER; i++) {
+                    const int r = i * (32 / PER) + lane / PER;
+                    const int64_t at = __shfl_sync(~0u, q_at, r);
+                    v[i] = r < rows_left && j < chunks ? __ldg((const uint4 *)((const T *)p.q + at) + j) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const int r = i * (32 / PER) + lane / PER;
+                    v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
+                    *(uint4 *)(dst + r * 128 + (j / 8) * QCHUNK + (((j & 7) ^ (r & 7)) << 4)) = v[i];
                 }
                 fence_async_smem();
                 mbar_arrive(&sh.q_ready[st]);
             }
             float m = -INFINITY, l = 0.0f;
-            const bool live = g.t1 * TK <= len.cached || (real && node_live(parent, node));
-            for (int i = DUAL ? 0 : st; i < n; i += DUAL ? 1 : 2) {
-                const int j0 = (g.t0 + i) * TK;
+            bool live = true;
+            uint64_t path = 0, alive = 0;  // up to 64 nodes: this row's path, and the nodes that are no padding
+            if (edges && p.n_node <= 64) {
+                warp_paths(parent_of, p.n_node, node, path, alive);
+                if (len.keys - len.past < 64) path &= len.keys > len.past ? (1ull << (len.keys - len.past)) - 1 : 0;
+                live = real && (alive >> node & 1);
+            } else if (edges) {
+                load_tree(sh.up[st], parent, p.n_node);
+                live = walk_tree(sh.up[st], real ? node : -2, [](int) {});
+                __syncwarp();
+            }
+            for (int i = 0; i < n; i++) {
+                const int j0 = (g.t0 + (DUAL ? i : 2 * i + st)) * TK;
                 const bool edge = j0 + TK > len.cached;  // not all of its keys are cached ones
-                uint32_t sees[4] = {~0u, ~0u, ~0u, ~0u};
+                constexpr int MW = (TK + 31) / 32;
+                uint32_t sees[MW];  // the keys this row sees
+#pragma unroll
+                for (int w = 0; w < MW; w++) sees[w] = ~0u;
                 if (edge) {
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
+                    for (int w = 0; w < MW; w++) {
                         const int k = len.cached - j0 - 32 * w;
                         sees[w] = !live ? 0u : k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1u;
                     }
-                    for (int j = live ? node : -1; j >= 0; j = node_up(parent, j)) {
-                        const int64_t at = (int64_t)len.past + j - j0;
-                        if (at < 0 || at >= TK || len.past + (int64_t)j >= p.max_seq) continue;
+                    if (p.n_node <= 64) {
+                        const uint64_t mine = live ? path : 0;
+                        const int at = len.past - j0;  // of node 0, from -63 on where any is in this tile
 #pragma unroll
-                        for (int w = 0; w < 4; w++)
-                            if (at >> 5 == w) sees[w] |= 1u << (at & 31);
+                        for (int w = 0; w < MW; w++) {
+                            const int up = at - 32 * w;
+                            if (up >= 0 && up < 32) sees[w] |= (uint32_t)(mine << up);
+                            if (up < 0 && up > -64) sees[w] |= (uint32_t)(mine >> -up);
+                        }
+                    } else {
+                        walk_tree(sh.up[st], live && real ? node : -1, [&](int j) {
+                            const int64_t row_at = (int64_t)len.past + j, at = row_at - j0;
+                            if (at < 0 || at >= TK || row_at >= p.max_seq) return;
+#pragma unroll
+                            for (int w = 0; w < MW; w++)
+                                if (at >> 5 == w) sees[w] |= 1u << (at & 31);
+                        });
+                        __syncwarp();
                     }
-                    // this thread's V row: nothing of it may meet a weight of zero unless it is finite
-                    const int vp = base + v_pos<DUAL>(i, n);
-                    if (!(ok = warp_wait(&sh.full[vp % NS], vp / NS & 1, &sh))) break;
-                    const int j = j0 + tid;
-                    if (j >= len.cached) {
-                        uint4 *v = (uint4 *)(ring + vp % NS * TILE + tid * 128);
-                        const bool gone = j >= len.keys || !node_live(parent, j - len.past);
+                    // The warp's V rows: nothing of them may meet a weight of zero unless it is finite.
+                    const int vp = base + 2 * i + 1, slot = (DUAL ? 0 : st * NS) + vp % NS;
+                    if (!(ok = warp_wait(&sh.full[slot], vp / NS & 1))) break;
+                    const int j = j0 + tid, d = j - len.past;
+                    const bool drafted = j >= len.cached && j < len.keys;
+                    const bool keep = tid >= TK || j < len.cached || (drafted && (p.n_node <= 64 ? alive >> d & 1 : walk_tree(sh.up[st], d, [](int) {})));
+                    const uint32_t gone = ~__ballot_sync(~0u, keep), look = __ballot_sync(~0u, tid < TK && drafted && keep);
+                    if (gone | look) {
+                        constexpr int PER = HC * 8;  // lanes to a row: 16 bytes each
+                        const int e = lane % PER;
+                        uint4 *v = (uint4 *)(ring + slot * TILE + (warp % 4) * 32 * 128 + (e / 8) * CHUNK) + (e & 7);
+                        uint32_t bad = 0;
 #pragma unroll
-                        for (int e = 0; e < HC * 8; e++) {
-                            uint4 *at = v + (e / 8) * (CHUNK / 16) + (e & 7);
-                            const uint4 x = *at;
-                            const uint4 y = gone ? make_uint4(0, 0, 0, 0)
-                                                 : make_uint4(finite2<T>(x.x), finite2<T>(x.y), finite2<T>(x.z), finite2<T>(x.w));
-                            if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
-                                *at = y;
-                                if (!gone) *(volatile int *)&sh.odd = seg + 1;
+                        for (int r = lane / PER; r < 32; r += 32 / PER) {
+                            if (look >> r & 1) {
+                                const uint4 x = v[8 * r];
+                                bad |= infinite2<T>(x.x) | infinite2<T>(x.y) | infinite2<T>(x.z) | infinite2<T>(x.w);
+                            } else if (gone >> r & 1) {
+                                v[8 * r] = make_uint4(0, 0, 0, 0);
                             }
                         }
+                        if (__any_sync(~0u, bad)) {
+                            for (int r = lane / PER; r < 32; r += 32 / PER)
+                                if (look >> r & 1) {
+                                    const uint4 x = v[8 * r];
+                                    v[8 * r] = make_uint4(finite2<T>(x.x), finite2<T>(x.y), finite2<T>(x.z), finite2<T>(x.w));
+                                }
+                            *(volatile int *)&sh.odd = seg + 1;
+                        }
+                        __syncwarp();
                     }
                     fence_async_smem();
                 }
-                if (!(ok = warp_wait(&sh.s_full[st], s_parity, &sh))) break;
+                if (!(ok = warp_wait(&sh.s_full[st], s_parity))) break;
                 s_parity ^= 1;
                 fence_after();
                 if (busy) {
                     float s[TK];
 #pragma unroll
-                    for (int w = 0; w < 4; w++) tmem_ld(tm_s + 32 * w, s + 32 * w);
+                    for (int k = 0; k < TK; k += 32) tmem_ld(tm_s + k, s + k);
                     tmem_ld_wait();
                     if (edge) {
 #pragma unroll
@@ -409,40 +509,42 @@ __global__ void __launch_bounds__(TT, 1)
                         const float f = m == -INFINITY ? 0.0f : exp2_fast(m - top);
                         l *= f;
                         m = top;
-                        if (i >= (DUAL ? 1 : 2)) {  // O holds something (the S that has arrived came after the last P V)
-                            for (int d = 0; d < n_pv; d += 32) {
-                                float o[32];
-                                tmem_ld(tm_o + d, o);
+                        if (i) {  // O holds something (the S that has arrived came after the last P V)
+                            for (int d = 0; d < n_pv; d += 16) {
+                                float o[16];
+                                tmem_ld16(tm_o + d, o);
                                 tmem_ld_wait();
 #pragma unroll
-                                for (int e = 0; e < 32; e++) o[e] *= f;
-                                tmem_st(tm_o + d, (const uint32_t *)o);
+                                for (int e = 0; e < 16; e++) o[e] *= f;
+                                tmem_st16(tm_o + d, (const uint32_t *)o);
                             }
                         }
                     }
                     const float off = m == -INFINITY ? 0.0f : m;
                     float l0 = 0.0f, l1 = 0.0f, l2 = 0.0f, l3 = 0.0f;
-                    uint32_t w[TK / 2];
 #pragma unroll
-                    for (int k = 0; k < TK; k += 4) {
-                        const float e0 = exp2_fast(fmaf(s[k], c, -off)), e1 = exp2_fast(fmaf(s[k + 1], c, -off));
-                        const float e2 = exp2_fast(fmaf(s[k + 2], c, -off)), e3 = exp2_fast(fmaf(s[k + 3], c, -off));
-                        l0 += e0, l1 += e1, l2 += e2, l3 += e3;
-                        w[k / 2] = pack2<T>(e0, e1);
-                        w[k / 2 + 1] = pack2<T>(e2, e3);
+                    for (int b = 0; b < TK; b += 32) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int k = b; k < b + 32; k += 4) {
+                            const float e0 = exp2_fast(fmaf(s[k], c, -off)), e1 = exp2_fast(fmaf(s[k + 1], c, -off));
+                            const float e2 = exp2_fast(fmaf(s[k + 2], c, -off)), e3 = exp2_fast(fmaf(s[k + 3], c, -off));
+                            l0 += e0, l1 += e1, l2 += e2, l3 += e3;
+                            w[(k - b) / 2] = pack2<T>(e0, e1);
+                            w[(k - b) / 2 + 1] = pack2<T>(e2, e3);
+                        }
+                        tmem_st16(tm_s + b / 2, w);
                     }
                     l += (l0 + l1) + (l2 + l3);
-                    tmem_st(tm_s, w);
-                    tmem_st(tm_s + 32, w + 32);
                     tmem_st_wait();
                 }
                 fence_before();
                 mbar_arrive(&sh.p_ready[st]);
             }
             if (!ok) break;
-            // the segment's end: O of this stream, or of both, is complete
-            if (DUAL || st < n) {
-                if (!(ok = warp_wait(&sh.o_done[st], o_parity, &sh))) break;
+            // the segment's end: O of this stream, then of both, is complete
+            if (n) {
+                if (!(ok = warp_wait(&sh.o_done[st], o_parity))) break;
                 o_parity ^= 1;
             }
             fence_after();
@@ -452,12 +554,12 @@ __global__ void __launch_bounds__(TT, 1)
                     sh.ml[tid] = make_float2(m, l);
                     fence_before();
                     mbar_arrive(&sh.merge_full);
-                    if (!(ok = warp_wait(&sh.merge_done, seg & 1, &sh))) break;
+                    if (!(ok = warp_wait(&sh.merge_done, seg & 1))) break;
                     seg++;
                     base += 2 * n;
                     continue;
                 }
-                if (!(ok = warp_wait(&sh.merge_full, seg & 1, &sh))) break;
+                if (!(ok = warp_wait(&sh.merge_full, seg & 1))) break;
                 fence_after();
                 const float2 other = sh.ml[tid];
                 const float top = fmaxf(m, other.x);
@@ -473,7 +575,7 @@ __global__ void __launch_bounds__(TT, 1)
                 const bool odd = *(volatile int *)&sh.odd == seg + 1;
                 const float inv = whole ? (live && l != 0.0f ? 1.0f / l : 0.0f) : 1.0f;
                 if (real && !whole) part_ml[slot * ROWS + in_group] = make_float2(m, live ? l : -1.0f);
-                T *out = (T *)p.out + g.s * p.out_seq + node * p.out_node + head * p.out_head;
+                uint8_t *stage = qbuf + (DUAL ? st : 0) * QTILE + (warp % 4) * 32 * 128;  // the rows of Q, no longer needed
                 for (int d = 0; d < p.head_dim; d += 32) {
                     float o[32], o1[32];
                     __syncwarp();
@@ -485,9 +587,9 @@ __global__ void __launch_bounds__(TT, 1)
                         o[e] = f == 0.0f ? 0.0f : o[e] * f;
                         if (!DUAL && f1 != 0.0f) o[e] += o1[e] * f1;
                     }
-                    if (odd && live) {  // what this row sees of the values that were left out
+                    if (odd) {  // what this row sees of the values that were left out
                         const T *v = (const T *)p.v_cache + g.s * p.cache_seq + g.head * p.cache_head + d;
-                        for (int j = node; j >= 0; j = node_up(parent, j)) {
+                        for (int j = live && real ? node : -1; j >= 0; j = node_up(parent, j)) {
                             const int64_t r = (int64_t)len.past + j;
                             if (r < (int64_t)g.t0 * TK || r >= (int64_t)g.t1 * TK || r >= p.max_seq) continue;
 #pragma unroll
@@ -497,25 +599,48 @@ __global__ void __launch_bounds__(TT, 1)
                             }
                         }
                     }
-                    if (real && whole) {
+                    if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            if (d + e < p.head_dim) {
-                                // a padding node's zero, whatever its sums hold
+                        for (int e = 0; e < 32; e += 8) {
+                            // a padding node's zero, whatever its sums hold
 #pragma unroll
-                                for (int b = 0; b < 8; b++) o[e + b] = inv == 0.0f ? 0.0f : o[e + b] * inv;
-                                *(uint4 *)(out + d + e) = make_uint4(pack2<T>(o[e], o[e + 1]), pack2<T>(o[e + 2], o[e + 3]),
-                                                                     pack2<T>(o[e + 4], o[e + 5]), pack2<T>(o[e + 6], o[e + 7]));
-                            }
-                    } else if (real) {
-                        float4 *dst = (float4 *)part_o + (slot * (p.head_dim / 4) + d / 4) * ROWS + in_group;
+                            for (int b = 0; b < 8; b++) o[e + b] = inv == 0.0f ? 0.0f : o[e + b] * inv;
+                            const int piece = (d + e) / 8;
+                            *(uint4 *)(stage + lane * 128 + (piece / 8) * QCHUNK + (((piece & 7) ^ (lane & 7)) << 4)) =
+                                make_uint4(pack2<T>(o[e], o[e + 1]), pack2<T>(o[e + 2], o[e + 3]), pack2<T>(o[e + 4], o[e + 5]),
+                                           pack2<T>(o[e + 6], o[e + 7]));
+                        }
+                    } else {  // 32 elements of 32 rows through shared memory, so that rows are written in runs
+                        __syncwarp();
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
-                            if (d + e < p.head_dim) dst[(e / 4) * ROWS] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            *(float4 *)(stage + lane * 128 + (((e / 4) ^ (lane & 7)) << 4)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        __syncwarp();
+                        const int e = lane % 8, rows_left = rows - (row - lane);
+                        float *dst = part_o + slot * part_stride(ROWS, p.head_dim) + (int64_t)(in_group - lane) * p.head_dim + d + 4 * e;
+                        if (d + 4 * e < p.head_dim)
+#pragma unroll
+                            for (int r = lane / 8; r < 32; r += 4)
+                                if (r < rows_left)
+                                    *(float4 *)(dst + r * p.head_dim) = *(const float4 *)(stage + r * 128 + ((e ^ (r & 7)) << 4));
                     }
                 }
             }
             __syncwarp();
+            if (busy && g.t0 == 0 && g.t1 == g.tiles) {
+                constexpr int PER = HC * 8;
+                const uint8_t *src = qbuf + (DUAL ? st : 0) * QTILE + (warp % 4) * 32 * 128;
+                const int64_t o_at = g.s * p.out_seq + node * p.out_node + head * p.out_head;
+                const int j = lane % PER, rows_left = rows - (row - lane);
+#pragma unroll
+                for (int i = 0; i < PER; i++) {
+                    const int r = i * (32 / PER) + lane / PER;
+                    const int64_t at = __shfl_sync(~0u, o_at, r);
+                    const uint4 v = *(const uint4 *)(src + r * 128 + (j / 8) * QCHUNK + (((j & 7) ^ (r & 7)) << 4));
+                    if (r < rows_left && j < chunks) *((uint4 *)((T *)p.out + at) + j) = v;
+                }
+                __syncwarp();
+            }
             fence_before();
             if (!DUAL) mbar_arrive(&sh.merge_done);
             seg++;
@@ -565,7 +690,7 @@ template <class T, bool DUAL, int HC>
 void tc_launch(const sdy_tree_attention_args &a, const TreeSpace &sp, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     smem_limit_once(tree_tc_kernel<T, DUAL, HC>, tc_smem(DUAL, HC), done);
-    launch(tree_tc_kernel<T, DUAL, HC>, TA_CTAS, TT, tc_smem(DUAL, HC), s, a, k, v, sp.base, sp.o, sp.ml);
+    launch(tree_tc_kernel<T, DUAL, HC>, TA_CTAS, TT, tc_smem(DUAL, HC), s, a, k, v, sp.cuts, sp.o, sp.ml);
     SDY_LAUNCHED();
 }
 template <class T>
@@ -591,7 +716,7 @@ void tree_tc(const sdy_tree_attention_args &a, cudaStream_t s) {
     const TreeSpace sp = tree_space(a, tree_tc_rows(a));
     if (a.type == T_F16) tc_pick<__half>(a, sp, k, v, s);
     else tc_pick<__nv_bfloat16>(a, sp, k, v, s);
-    tree_join(a, sp, tree_tc_rows(a), TA_CTAS, s);
+    tree_join(a, sp, tree_tc_rows(a), s);
 }
 
 unsigned tree_tc_status() {
