@@ -48,7 +48,7 @@ constexpr int tc_smem(bool dual, int hc) { return (dual ? 2 : 1) * hc * QCHUNK +
 struct Shared {
     uint64_t full[SLOTS], empty[SLOTS];
     uint64_t q_ready[2], s_full[2], p_ready[2], o_done[2];
-    uint64_t merge_full, merge_done, drain[2];
+    uint64_t merge_full, merge_done, drain;
     uint32_t tmem;
     int odd;  // the last segment (from 1) whose drafted V rows hold NaN or infinities
     int64_t scan[TT / 32], share[7];
@@ -240,12 +240,12 @@ __global__ void __launch_bounds__(TT, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < NS * STEP; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], NQ);
+        for (int i = 0; i < NS * STEP; i++) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sh.q_ready[i], TR), mbar_init(&sh.s_full[i], 1);
             mbar_init(&sh.p_ready[i], TR), mbar_init(&sh.o_done[i], 1);
         }
-        mbar_init(&sh.merge_full, TR), mbar_init(&sh.merge_done, TR), mbar_init(&sh.drain[0], 1), mbar_init(&sh.drain[1], 1);
+        mbar_init(&sh.merge_full, TR), mbar_init(&sh.merge_done, TR), mbar_init(&sh.drain, 1);
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         sh.odd = 0;
     }
@@ -258,35 +258,46 @@ __global__ void __launch_bounds__(TT, 1)
     Share<TK> share(p, sh.share, p.n_kv_head * groups);
     Segment g;
 
-    // registers go to the two warpgroups that hold rows: 96 x 128 + 200 x 256 <= 168 x 384
+    // registers go to the two warpgroups that hold rows: 72 x 128 + 216 x 256 <= 168 x 384
     if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 96;\n" ::);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n" ::);
         if (warp == 0 && lane == 0) {
-            int pos[STEP] = {};  // loads so far, per ring
-            bool ok = true;
-            auto load = [&](const CUtensorMap *map, int r, int i) {  // the stream's tile i into ring r
+            int pos[STEP] = {}, event[STEP] = {};  // loads and arrivals so far, per ring
+            bool ok = true, begun = false;
+            // the stream's tile i into the next slot of ring r, with `bytes` more to come on the arrival
+            auto load = [&](const CUtensorMap *map, int r, int i, int bytes) {
                 const int slot = r * NS + pos[r] % NS, turn = pos[r] / NS;
+                uint64_t *full = &sh.full[r * NS + event[r] % NS];
                 if (turn && !mbar_wait(&sh.empty[slot], (turn - 1) & 1)) return false;
-                // the first queries do not queue behind rings full of tiles
-                if (r == 0 && pos[0] == 1 && !(mbar_wait(&sh.q_ready[0], 0) && (!DUAL || mbar_wait(&sh.q_ready[1], 0)))) return false;
-                mbar_expect(&sh.full[slot], TILE);
+                if (bytes) mbar_expect(full, bytes);
                 for (int c = 0; c < HC; c++)
-                    tma_tile(map, &sh.full[slot], smem_u32(ring + slot * TILE + c * CHUNK), 64 * c, (g.t0 + i * STEP + r) * TK, g.head, g.s);
+                    tma_tile(map, full, smem_u32(ring + slot * TILE + c * CHUNK), 64 * c, (g.t0 + i * STEP + r) * TK, g.head, g.s);
                 pos[r]++;
                 return true;
             };
             while (ok && share.next(g, groups)) {
                 const int n = g.t1 - g.t0;
-                for (int i = 0; ok && i < n; i += STEP) {
 #pragma unroll
-                    for (int r = 0; r < STEP; r++)
-                        if (i + r < n) ok = ok && load(&kmap, r, i / STEP) && load(&vmap, r, i / STEP);
+                for (int r = 0; r < STEP; r++)
+                    if (r < n) ok = ok && load(&kmap, r, 0, TILE), event[r]++;
+                // the first queries do not queue behind rings full of tiles
+                if (!begun) ok = ok && mbar_wait(&sh.q_ready[0], 0) && (!DUAL || mbar_wait(&sh.q_ready[1], 0));
+                begun = true;
+                for (int i = 0; ok && i * STEP < n; i++) {
+#pragma unroll
+                    for (int r = 0; r < STEP; r++) {  // V, and the K that follows it, arrive together
+                        if (i * STEP + r >= n) continue;
+                        const bool more = (i + 1) * STEP + r < n;
+                        ok = ok && load(&vmap, r, i, more ? 2 * TILE : TILE);
+                        if (more) ok = ok && load(&kmap, r, i + 1, 0);
+                        event[r]++;
+                    }
                 }
             }
             if (!ok) {  // let the copies in flight land before the memory is given up
                 atomicOr(&g_tree_status, 1u);
                 for (int r = 0; r < STEP; r++)
-                    for (int q = max(0, pos[r] - NS); q < pos[r]; q++) mbar_wait(&sh.full[r * NS + q % NS], q / NS & 1);
+                    for (int q = max(0, event[r] - NS); q < event[r]; q++) mbar_wait(&sh.full[r * NS + q % NS], q / NS & 1);
             }
         }
         if (warp == 3 && lane == 0) note_cut<TK>(p, p.n_kv_head * groups, groups, blockIdx.x, sh.share, cuts);
@@ -300,78 +311,85 @@ __global__ void __launch_bounds__(TT, 1)
                 }
             }
         }
-        if (warp == 1 || warp == 2) {
-            // A warp issues for one stream: a wait on a barrier that is complete takes 100 cycles and the
-            // tensor pipe queues little, so with one warp for both it would idle during every wait. The
-            // whole warp waits, one lane issues; the shuffles tell the compiler that the operands are the
-            // same in all lanes (the tensor instructions take them from uniform registers).
+        if (warp == 1) {
+            // One warp issues for both streams in turn, which keeps them out of step: the one's MMAs run
+            // under the other's exponentials (with a warp for each they fall into step and share both
+            // pipes: 4600 cycles per unit instead of 3600). The whole warp waits, one lane issues; the
+            // shuffles tell the compiler that the operands are the same in all lanes (the tensor
+            // instructions take them from uniform registers).
             auto uniform = [](uint32_t x) { return __shfl_sync(~0u, x, 0); };
-            const int st = (int)uniform(warp - 1), first_slot = DUAL ? 0 : st * NS;
             const uint32_t id_qk = uniform(idesc_f16(BF, TK, false)), id_pv = uniform(idesc_f16(BF, n_pv, true));
-            const uint32_t q_lo = uniform(desc_lo(smem_u32(qbuf + (DUAL ? st : 0) * QTILE), 16)), steps = uniform(k_steps);
+            const uint32_t q_lo = uniform(desc_lo(smem_u32(qbuf), 16)), steps = uniform(k_steps), tm = uniform(tmem);
             const uint32_t k_lo = uniform(desc_lo(smem_u32(ring), 16)), v_lo = uniform(desc_lo(smem_u32(ring), CHUNK));
-            const uint32_t tm_s = uniform(tmem) + TM_S + st * 128, tm_o = tm_s - TM_S + TM_O;
-            int base = 0, seg = 0;  // ring position of the segment's first load, segments so far
+            int pos[2] = {}, event[2] = {}, seg = 0;  // loads and arrivals taken, per stream; segments so far
             uint32_t p_parity = 0;
             bool ok = true;
-            auto slot_of = [&](int pos) { return first_slot + pos % NS; };
-            auto wait_full = [&](int pos) { return warp_wait(&sh.full[slot_of(pos)], pos / NS & 1); };
-            auto qk = [&](int pos) {
-                const uint32_t b = uniform(k_lo + slot_of(pos) * (TILE >> 4));
+            auto slot_of = [&](int st, int at) { return (DUAL ? 0 : st * NS) + at % NS; };
+            auto wait_full = [&](int st, int e) { return warp_wait(&sh.full[slot_of(st, e)], e / NS & 1); };
+            auto qk = [&](int st, uint32_t b, uint64_t *free) {
+                const uint32_t a = q_lo + (DUAL ? st : 0) * (QTILE >> 4), d = tm + TM_S + st * 128;
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < 4 * HC; k++)
                         if (k < steps)
-                            mma_ss(tm_s, q_lo + (((k / 4) * QCHUNK + (k % 4) * 32) >> 4), b + (((k / 4) * CHUNK + (k % 4) * 32) >> 4), id_qk, k > 0);
+                            mma_ss(d, a + (((k / 4) * QCHUNK + (k % 4) * 32) >> 4), b + (((k / 4) * CHUNK + (k % 4) * 32) >> 4), id_qk, k > 0);
                     mma_commit(&sh.s_full[st]);
-                    mma_commit(&sh.empty[slot_of(pos)]);
-                }
-            };
-            auto pv = [&](int pos, bool first) {
-                const uint32_t b = uniform(v_lo + slot_of(pos) * (TILE >> 4)), again = uniform(!first);
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < TK / 16; k++) mma_ts(tm_o, tm_s + 8 * k, b + (2048 * k >> 4), id_pv, k > 0 ? 1u : again);
-                    mma_commit(&sh.empty[slot_of(pos)]);
+                    if (!DUAL || st == 1) mma_commit(free);
                 }
             };
             while (ok && share.next(g, groups)) {
-                const int n = (g.t1 - g.t0 + STEP - 1 - (DUAL ? 0 : st)) / STEP;  // the stream's tiles
-                if (!(ok = warp_wait(&sh.q_ready[DUAL ? st : 0], seg & 1))) break;
+                const int all = g.t1 - g.t0;
+                auto tiles = [&](int st) { return DUAL ? all : (all + 1 - st) / 2; };  // of a stream
+                for (int st = 0; ok && st < NQ; st++) ok = warp_wait(&sh.q_ready[st], seg & 1);
                 fence_after();
-                if (n) {
-                    if (!(ok = wait_full(base))) break;
-                    qk(base);
+#pragma unroll
+                for (int st = 0; st < 2; st++) {
+                    if (!ok || !tiles(st)) continue;
+                    const int slot = slot_of(st, pos[st]);
+                    if ((ok = wait_full(st, event[st]))) qk(st, uniform(k_lo + slot * (TILE >> 4)), &sh.empty[slot]);
+                    pos[st]++, event[st]++;
                 }
-                for (int i = 0; i < n; i++) {
-                    const int pos = base + 2 * i + 1;
-                    // both tiles are waited for first: P is what comes last
-                    if (!(ok = wait_full(pos) && (i + 1 == n || wait_full(pos + 1)) && warp_wait(&sh.p_ready[st], p_parity))) break;
-                    p_parity ^= 1;
-                    fence_after();
-                    pv(pos, i == 0);
-                    if (i + 1 < n) qk(pos + 1);  // over P, which the MMAs before have read by then
-                    else if (elect_one()) mma_commit(&sh.o_done[st]);
+                for (int i = 0; ok && i < tiles(0); i++) {
+#pragma unroll
+                    for (int st = 0; st < 2; st++) {
+                        if (!ok || i >= tiles(st)) continue;
+                        const bool more = i + 1 < tiles(st);
+                        const int v_slot = slot_of(st, pos[st]), k_slot = slot_of(st, pos[st] + 1);
+                        const uint32_t v = uniform(v_lo + v_slot * (TILE >> 4)), k = uniform(k_lo + k_slot * (TILE >> 4)), again = uniform(i > 0);
+                        if (!DUAL || st == 0) ok = wait_full(st, event[st]);
+                        pos[st] += more ? 2 : 1, event[st]++;
+                        ok = ok && warp_wait(&sh.p_ready[st], p_parity >> st & 1);
+                        if (!ok) continue;
+                        p_parity ^= 1u << st;
+                        fence_after();
+                        if (elect_one()) {
+                            const uint32_t d = tm + TM_O + st * 128, a = tm + TM_S + st * 128;
+#pragma unroll
+                            for (int c = 0; c < TK / 16; c++) mma_ts(d, a + 8 * c, v + (2048 * c >> 4), id_pv, c > 0 ? 1u : again);
+                            if (!DUAL || st == 1) mma_commit(&sh.empty[v_slot]);
+                            if (!more) mma_commit(&sh.o_done[st]);
+                        }
+                        if (more) qk(st, k, &sh.empty[k_slot]);  // over P, which the MMAs before have read by then
+                    }
                 }
-                base += 2 * n;
                 seg++;
             }
             if (!ok) {  // the MMAs in flight end before the tensor memory is freed
                 if (lane == 0) atomicOr(&g_tree_status, 1u);
-                if (elect_one()) mma_commit(&sh.drain[st]);
-                warp_wait(&sh.drain[st], 0);
+                if (elect_one()) mma_commit(&sh.drain);
+                warp_wait(&sh.drain, 0);
             }
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;\n" ::);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n" ::);
         const int st = (warp - 4) / 4, tid = threadIdx.x - 128 - 128 * st;  // stream, row of its tile
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;                  // 32 lanes to a warp
         const uint32_t tm_s = tmem + TM_S + st * 128 + lanes, tm_o = tmem + TM_O + st * 128 + lanes;
         const float c = fabsf(p.scale) * 1.4426950408889634f;
         const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
         const int chunks = p.head_dim / 8;  // 16-byte pieces of a row
-        int base = 0, seg = 0;
+        int base = 0, arrived = 0, seg = 0;  // loads, arrivals and segments before this one
         uint32_t s_parity = 0, o_parity = 0;
         bool ok = true;
         while (ok && share.next(g, groups)) {
@@ -453,8 +471,8 @@ __global__ void __launch_bounds__(TT, 1)
                         __syncwarp();
                     }
                     // The warp's V rows: nothing of them may meet a weight of zero unless it is finite.
-                    const int vp = base + 2 * i + 1, slot = (DUAL ? 0 : st * NS) + vp % NS;
-                    if (!(ok = warp_wait(&sh.full[slot], vp / NS & 1))) break;
+                    const int vp = base + 2 * i + 1, slot = (DUAL ? 0 : st * NS) + vp % NS, ve = arrived + 1 + i;
+                    if (!(ok = warp_wait(&sh.full[(DUAL ? 0 : st * NS) + ve % NS], ve / NS & 1))) break;
                     const int j = j0 + tid, d = j - len.past;
                     const bool drafted = j >= len.cached && j < len.keys;
                     const bool keep = tid >= TK || j < len.cached || (drafted && (p.n_node <= 64 ? alive >> d & 1 : walk_tree(sh.up[st], d, [](int) {})));
@@ -556,7 +574,7 @@ __global__ void __launch_bounds__(TT, 1)
                     mbar_arrive(&sh.merge_full);
                     if (!(ok = warp_wait(&sh.merge_done, seg & 1))) break;
                     seg++;
-                    base += 2 * n;
+                    base += 2 * n, arrived += n ? n + 1 : 0;
                     continue;
                 }
                 if (!(ok = warp_wait(&sh.merge_full, seg & 1))) break;
@@ -644,7 +662,7 @@ __global__ void __launch_bounds__(TT, 1)
             fence_before();
             if (!DUAL) mbar_arrive(&sh.merge_done);
             seg++;
-            base += 2 * n;
+            base += 2 * n, arrived += n ? n + 1 : 0;
         }
     }
     fence_before();
