@@ -10,15 +10,16 @@ constexpr int TA_MAX_NODES = 256;
 constexpr int TA_MAX_DIM = 256;
 
 // The split. A row group is the rows (node, query head) of one KV head of one sequence that a CTA
-// holds at once. Its work is its tiles of keys and TA_SETUP more units for loading the queries and
-// storing the result (which for short sequences is most of the time). The units of a call, sequence
+// holds at once. Its work is its tiles of keys and, unless every tile finds a CTA of its own,
+// TA_SETUP more units for loading the queries and storing the result (about as long as that many
+// tiles, most of the time of a short sequence). The units of a call, sequence
 // by sequence, KV head by KV head, row group by row group, are dealt to TA_CTAS CTAs in equal
 // contiguous shares, whatever the lengths of the sequences, which only the device knows. A CTA
 // writes the result of a row group whose tiles it holds all; of one that its share cuts it leaves
 // the unnormalised sum, the maximum and the sum of weights in one of its two slots of the workspace
 // (first and last row group of its share), and join_kernel adds them up in the order of the CTAs.
 constexpr int TA_CTAS = 148;  // one per SM
-constexpr int TA_SETUP = 3;
+constexpr int TA_SETUP = 6;
 
 // A row group to join, noted by the second CTA that holds tiles of it: the parts are the slot of
 // that CTA's predecessor and the first slots of the CTAs from it on.
@@ -100,32 +101,32 @@ template <int KEYS>
 struct Share {
     const sdy_tree_attention_args &p;
     int64_t u, end, base;   // next unit, end, units of the sequences before s
-    int s, tiles, past, items;  // items: row groups per sequence
+    int s, tiles, past, items, setup;  // items: row groups per sequence; setup: units before a group's tiles
     __device__ Share(const sdy_tree_attention_args &p_, const int64_t *found, int items_)
         : p(p_), u(found[0]), end(found[1]), base(found[3]), s((int)found[2]), tiles((int)found[4]),
-          past((int)found[6]), items(items_) {}
+          past((int)found[6]), items(items_), setup((int)found[7]) {}
     // The next run; runs that hold no tile (only the end of a row group's setup) are passed over.
     __device__ bool next(Segment &g, int groups) {
         while (u < end) {
-            while (u >= base + (int64_t)(tiles + TA_SETUP) * items) {
-                base += (int64_t)(tiles + TA_SETUP) * items;
+            while (u >= base + (int64_t)(tiles + setup) * items) {
+                base += (int64_t)(tiles + setup) * items;
                 s++;
                 past = max(p.n_past[s], 0);
                 tiles = (lengths_of(p, s, past).keys + KEYS - 1) / KEYS;
             }
             const int64_t r = u - base;
-            const int per = tiles + TA_SETUP, item = r >> 31 ? (int)(r / per) : (int)((unsigned)r / (unsigned)per);
+            const int per = tiles + setup, item = r >> 31 ? (int)(r / per) : (int)((unsigned)r / (unsigned)per);
             const int at = (int)(r - (int64_t)item * per);
             const int to = (int)min((int64_t)per, at + end - u);
             u += to - at;
-            if (to <= TA_SETUP) continue;
+            if (to <= setup) continue;
             g.s = s;
             g.head = item / groups;
             g.group = item - g.head * groups;
             g.tiles = tiles;
             g.past = past;
-            g.t0 = max(at - TA_SETUP, 0);
-            g.t1 = to - TA_SETUP;
+            g.t0 = max(at - setup, 0);
+            g.t1 = to - setup;
             return true;
         }
         return false;
@@ -134,7 +135,8 @@ struct Share {
 
 // Where CTA `cta`'s share begins, found by the whole block (THREADS threads, all of them): the
 // units before each run of sequences by a scan over the threads, the rest by walking that run.
-// out[0..6] = first unit, end, first sequence, units before it, its tiles, all units, its length.
+// out[0..7] = first unit, end, first sequence, units before it, its tiles, all units, its length, the
+// setup.
 template <int KEYS, int THREADS>
 __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int items, int cta,
                                            int64_t *scan /* THREADS / 32 */, int64_t *out) {
@@ -142,7 +144,7 @@ __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int
     const int s0 = min(t * run, p.n_seq), s1 = min(s0 + run, p.n_seq);
     auto tiles_of = [&](int s) { return (lengths_of(p, s).keys + KEYS - 1) / KEYS; };
     int64_t mine = 0;
-    for (int s = s0; s < s1; s++) mine += tiles_of(s) + TA_SETUP;
+    for (int s = s0; s < s1; s++) mine += tiles_of(s);
     int64_t sum = mine;  // inclusive over the warp
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t v = __shfl_up_sync(~0u, sum, o);
@@ -157,15 +159,17 @@ __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int
         if (w < t / 32) before += scan[w];
         total += scan[w];
     }
-    before += sum - mine;
-    const int64_t units = total * items;
+    const int setup = total * items <= TA_CTAS ? 0 : TA_SETUP;
+    before += sum - mine + (int64_t)s0 * setup;
+    mine += (int64_t)(s1 - s0) * setup;
+    const int64_t units = (total + (int64_t)p.n_seq * setup) * items;
     const int64_t u0 = share_begin(units, cta), u1 = share_begin(units, cta + 1);
-    if (t == 0) out[0] = u0, out[1] = u1, out[5] = units;
+    if (t == 0) out[0] = u0, out[1] = u1, out[5] = units, out[7] = setup;
     if (u0 < u1 && u0 >= before * items && u0 < (before + mine) * items) {
-        int s = s0, n = run == 1 ? (int)mine - TA_SETUP : tiles_of(s0);
+        int s = s0, n = run == 1 ? (int)mine - setup : tiles_of(s0);
         int64_t b = before * items;
-        while (u0 >= b + (int64_t)(n + TA_SETUP) * items) {
-            b += (int64_t)(n + TA_SETUP) * items;
+        while (u0 >= b + (int64_t)(n + setup) * items) {
+            b += (int64_t)(n + setup) * items;
             s++;
             n = tiles_of(s);
         }
@@ -182,11 +186,11 @@ __device__ __forceinline__ void note_cut(const sdy_tree_attention_args &p, int i
     Segment g;
     if (share.next(g, groups) && g.t0 > 0) {
         const int64_t units = found[5], item = g.head * groups + g.group;
-        const int64_t u0 = share.base + item * (g.tiles + TA_SETUP);
-        const int first = share_of(units, u0 + TA_SETUP);  // the CTA that holds the first tile
+        const int64_t u0 = share.base + item * (g.tiles + share.setup);
+        const int first = share_of(units, u0 + share.setup);  // the CTA that holds the first tile
         if (first == cta - 1) {
             cut.s = g.s, cut.item = (int)item;
-            cut.parts = share_of(units, u0 + TA_SETUP + g.tiles - 1) - first + 1;
+            cut.parts = share_of(units, u0 + share.setup + g.tiles - 1) - first + 1;
             cut.first_slot = 2 * first + (share_begin(units, first) < u0);
         }
     }

@@ -51,7 +51,7 @@ struct Shared {
     uint64_t merge_full, merge_done, drain;
     uint32_t tmem;
     int odd;  // the last segment (from 1) whose drafted V rows hold NaN or infinities
-    int64_t scan[TT / 32], share[7];
+    int64_t scan[TT / 32], share[8];
     int16_t up[2][TA_MAX_NODES];  // per stream (its warps are in one segment while they walk)
     float2 ml[TR];
 };
