@@ -3,30 +3,46 @@
 //
 // All filters keep a prefix of one order: the logits descending, equal ones by index. An entry of
 // that order is one 64-bit number, order(i) = key(logit_i) << 32 | ~i, with key the usual
-// order-preserving image of a float, so a filter is a lower bound on it: top-k's is the k-th
+// order-preserving image of a float, so a filter is a lower bound on it ("cut"): top-k's is the k-th
 // largest, top-p's the largest c with mass(order >= c) >= top_p * mass. Masses are integers:
 // w = exp((l - max) / T) in 64 bits, rounded to 2^-44, so that 400000 of them fit 64 bits and their
 // sum does not depend on the order of the additions. A 32-bit weight would be off by 2^-24 of
 // itself, enough to move a choice whose uniform number lies next to a border once in some ten
 // thousand rows; this leaves 10^-12.
+//
+// A cluster of up to eight CTAs holds a row in its shared memory, so the row is read once. A cut is
+// found by a histogram of the row's distance from its largest logit (1024 buckets of 1/32, in units
+// of the temperature), of numbers for top-k and masses for top-p, merged over the cluster; the
+// entries of the bucket where the count crosses are gathered and ranked in the first CTA. A bucket of
+// too many entries is split again by key, one of equal keys by index. Top-k comes first, so a top-p
+// after it takes exponentials of the kept entries alone; the last pass forms the masses of what is
+// kept in index order and finds the entry at the uniform number.
+//
+// Bound by latency for few rows (a dozen cluster barriers and passes over shared memory), for many by
+// the exponentials (64 bits: about 20 operations at half the 32-bit rate) and the passes.
 #include "draft.cuh"
 #include "sample.cuh"
 #include "sardyne_b200.h"
 
+#include <cooperative_groups.h>
 #include <math.h>
 
 namespace sdy {
+namespace cg = cooperative_groups;
 namespace {
 
-constexpr int S_THREADS = 1024;
+constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32;
 constexpr int S_MAX_VOCAB = SAMPLE_MAX_VOCAB;
+constexpr int S_CLUSTER = 8;                   // CTAs to a row, at most
+constexpr int S_BUCKETS = 1024, S_LIST = 1024;  // the list: entries ranked at once
+constexpr double S_SCALE = 32.0;               // buckets per unit of (max - l) / T
 constexpr unsigned KEY_NEG_INF = 0x007FFFFFu;  // key(-inf); NaN takes key 0
 constexpr double MASS_ONE = 17592186044416.0;  // 2^44
 typedef unsigned long long u64;
 
 __device__ __forceinline__ unsigned key_of(float x) {
     if (x != x) return 0;
-    const unsigned b = __float_as_uint(x);
+    const unsigned b = __float_as_uint(x + 0.0f);  // (-0 is the same logit as 0)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(unsigned key) {
@@ -43,104 +59,341 @@ struct Weight {
     __device__ u64 mass(unsigned key) const { return (u64)__double2ll_rn((*this)(key) * MASS_ONE); }
 };
 
-__device__ u64 block_sum(u64 v, u64 *part) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = part[threadIdx.x % 32];
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-    return v;
-}
-__device__ u64 block_max(u64 v, u64 *part) {
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = part[threadIdx.x % 32];
-    for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(~0u, v, o));
-    return v;
-}
+struct Sum {
+    u64 count, mass;
+    __device__ Sum operator+(const Sum &o) const { return {count + o.count, mass + o.mass}; }
+};
+__device__ __forceinline__ Sum shfl_up(Sum v, int o) { return {__shfl_up_sync(~0u, v.count, o), __shfl_up_sync(~0u, v.mass, o)}; }
+
+struct SampleShared {
+    unsigned count[S_BUCKETS], lo[S_BUCKETS], hi[S_BUCKETS];  // of this CTA's entries (mass in two words)
+    u64 list[S_LIST], sorted[S_LIST];                         // first CTA: gathered entries
+    unsigned n_list;
+    Sum part[S_WARPS + 1];                                    // per warp, then the CTA
+    Sum all[2][S_CLUSTER];                                    // exchanged, by rank; two in turn
+    u64 said[2][4];                                           // what one CTA tells the others; two in turn
+    u64 best;
+};
 
 template <class T>
-__global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args p) {
-    __shared__ u64 part[32];
-    __shared__ u64 before[S_THREADS];
-    pdl_wait();
-    const int64_t row = blockIdx.x;
-    const T *x = (const T *)p.logits + row * p.row_stride;
-    const int n = p.n_vocab;
-    auto key_at = [&](int i) { return key_of(to_f32(x[i])); };
+struct Sampler {
+    SampleShared &sh;
+    cg::cluster_group cl;
+    const T *x;     // this CTA's entries
+    int n, first;   // their number, the index of the first
+    int rank, ranks, tid, warp, lane;
+    int turn = 0, told = 0;
 
+    __device__ unsigned key(int i) const { return key_of(to_f32(x[i])); }
+
+    // v summed over the warps of the CTA up to and with this thread's; the CTA's sum in sh.part[S_WARPS].
+    __device__ Sum scan(Sum v) {
+        Sum in = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const Sum u = shfl_up(in, o);
+            if (lane >= o) in = in + u;
+        }
+        __syncthreads();
+        if (lane == 31) sh.part[warp] = in;
+        __syncthreads();
+        if (warp == 0) {
+            Sum w = lane < S_WARPS ? sh.part[lane] : Sum{0, 0}, t = w;
+            for (int o = 1; o < S_WARPS; o <<= 1) {
+                const Sum u = shfl_up(t, o);
+                if (lane >= o) t = t + u;
+            }
+            __syncwarp();
+            if (lane < S_WARPS) sh.part[lane] = {t.count - w.count, t.mass - w.mass};
+            if (lane == S_WARPS - 1) sh.part[S_WARPS] = t;
+        }
+        __syncthreads();
+        return sh.part[warp] + in;
+    }
+    // The sums of the CTAs of lower rank and of all, from every CTA's sum in sh.part[S_WARPS].
+    __device__ void exchange(Sum &before, Sum &total) {
+        if (tid < ranks) cl.map_shared_rank(&sh, tid)->all[turn][rank] = sh.part[S_WARPS];
+        cl.sync();
+        before = total = {0, 0};
+        for (int r = 0; r < ranks; r++) {
+            if (r < rank) before = before + sh.all[turn][r];
+            total = total + sh.all[turn][r];
+        }
+        turn ^= 1;
+    }
+    // Four numbers from the one CTA in which one thread's `mine` is set, to all.
+    __device__ void tell(bool mine, const u64 (&v)[4], u64 (&got)[4]) {
+        if (mine)
+            for (int r = 0; r < ranks; r++)
+                for (int i = 0; i < 4; i++) cl.map_shared_rank(&sh, r)->said[told][i] = v[i];
+        cl.sync();
+        for (int i = 0; i < 4; i++) got[i] = sh.said[told][i];
+        told ^= 1;
+    }
+
+    // The index at which the running sum of f(i), in index order, passes `want_of(total)`; the sum of
+    // all and the f there in `total` and `at`.
+    template <class F, class W>
+    __device__ int locate(F f, W want_of, u64 &total, u64 &at) {
+        // a warp's entries are a run of indexes
+        const int per = (n + S_WARPS * 32 - 1) / (S_WARPS * 32) * 32, i0 = min(warp * per, n), i1 = min(i0 + per, n);
+        u64 mine = 0;
+        for (int i = i0 + lane; i < i1; i += 32) mine += f(i);
+        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
+        const Sum to = scan({0, lane == 31 ? mine : 0});
+        Sum before, sum;
+        exchange(before, sum);
+        total = sum.mass;
+        const u64 want = want_of(total), end = before.mass + __shfl_sync(~0u, to.mass, 31), begin = end - mine;
+        bool mine_it = false;
+        u64 v[4] = {0, 0, 0, 0};
+        if (want >= begin && want < end) {
+            u64 c = begin;
+            for (int i = i0;; i += 32) {
+                const u64 m = i + lane < i1 ? f(i + lane) : 0;
+                u64 in = m;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 u = __shfl_up_sync(~0u, in, o);
+                    if (lane >= o) in += u;
+                }
+                const unsigned past = __ballot_sync(~0u, want < c + in);
+                if (past) {
+                    mine_it = lane == __ffs(past) - 1;
+                    v[0] = first + i + lane, v[1] = m;
+                    break;
+                }
+                c += __shfl_sync(~0u, in, 31);
+            }
+        }
+        u64 got[4];
+        tell(mine_it, v, got);
+        at = got[1];
+        return (int)got[0];
+    }
+
+    // The lowest order of the shortest prefix whose number (MASS: mass) reaches target_of(the sum of
+    // all entries from `cut` on).
+    template <bool MASS, class Target>
+    __device__ u64 find_cut(const Weight &weight, u64 cut, Target target_of) {
+        unsigned k_hi = weight.top, k_lo = 0;  // the keys in question (k_lo 0: by distance, else by key)
+        int shift = 0;
+        Sum done = {0, 0};                     // before them
+        u64 target = 0;
+        for (int level = 0;; level++) {
+            auto bucket = [&](unsigned key) -> int {
+                if (level) return (int)((k_hi - key) >> shift);
+                if (key == weight.top) return 0;
+                return (int)fmin((weight.m - (double)value_of(key)) * weight.inv * S_SCALE, S_BUCKETS - 1.0);
+            };
+            for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
+            if (tid == 0) sh.n_list = 0;
+            __syncthreads();
+            unsigned far = 0;  // entries in the last bucket, which has most of them (at level 0 they have no mass)
+            for (int i = tid; i < n; i += S_THREADS) {
+                const unsigned k = key(i);
+                if (k <= KEY_NEG_INF || order_of(k, first + i) < cut || (level && (k < k_lo || k > k_hi))) continue;
+                const int b = bucket(k);
+                if (b == S_BUCKETS - 1 && !level) {
+                    far++;
+                    continue;
+                }
+                atomicAdd(&sh.count[b], 1u);
+                if (MASS) {
+                    const u64 m = weight.mass(k);
+                    const unsigned low = (unsigned)m, old = atomicAdd(&sh.lo[b], low);
+                    const unsigned high = (unsigned)(m >> 32) + (old + low < low);
+                    if (high) atomicAdd(&sh.hi[b], high);
+                }
+            }
+            for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(~0u, far, o);
+            if (lane == 0 && far) atomicAdd(&sh.count[S_BUCKETS - 1], far);
+            cl.sync();
+            // this CTA merges a run of buckets, two to a thread at most
+            const int run = S_BUCKETS / ranks, per = (run + S_THREADS - 1) / S_THREADS, b0 = rank * run + tid * per;
+            Sum own[2] = {{0, 0}, {0, 0}};
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                if (j < per && tid * per + j < run)
+                    for (int r = 0; r < ranks; r++) {
+                        const SampleShared *o = cl.map_shared_rank(&sh, r);
+                        own[j] = own[j] + Sum{o->count[b0 + j], (u64)o->hi[b0 + j] << 32 | o->lo[b0 + j]};
+                    }
+            const Sum to = scan(own[0] + own[1]);
+            Sum before, total;
+            exchange(before, total);
+            if (!level) target = target_of(total);
+            // the bucket in which the sum reaches the target
+            bool here = false;
+            u64 v[4] = {0, 0, 0, 0};
+            Sum c = done + before + to;
+            c = {c.count - own[0].count - own[1].count, c.mass - own[0].mass - own[1].mass};
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const u64 from = MASS ? c.mass : c.count;
+                const Sum next = c + own[j];
+                if (!here && from < target && target <= (MASS ? next.mass : next.count)) {
+                    here = true;
+                    v[0] = b0 + j, v[1] = c.count, v[2] = c.mass, v[3] = own[j].count;
+                }
+                c = next;
+            }
+            u64 got[4];
+            tell(here, v, got);
+            const int crossing = (int)got[0];
+            done = {got[1], got[2]};
+            if (got[3] <= S_LIST) {
+                // gathered and ranked in the first CTA: every entry counts the ones before it
+                SampleShared *lead = cl.map_shared_rank(&sh, 0);
+                for (int i = tid; i < n; i += S_THREADS) {
+                    const unsigned k = key(i);
+                    if (k <= KEY_NEG_INF || order_of(k, first + i) < cut || (level && (k < k_lo || k > k_hi)) || bucket(k) != crossing)
+                        continue;
+                    lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(k, first + i);
+                }
+                cl.sync();
+                bool found = false;
+                u64 w[4] = {0, 0, 0, 0};
+                if (rank == 0) {
+                    const int m = (int)got[3];
+                    for (int i = tid; i < m; i += S_THREADS) {
+                        const u64 mine = sh.list[i];
+                        int at = 0;
+                        for (int j = 0; j < m; j++) at += sh.list[j] > mine;
+                        sh.sorted[at] = mine;
+                    }
+                    __syncthreads();
+                    Sum e[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int i = 2 * tid + j;
+                        e[j] = i < m ? Sum{1, MASS ? weight.mass((unsigned)(sh.sorted[i] >> 32)) : 0} : Sum{0, 0};
+                    }
+                    const Sum upto = done + scan(e[0] + e[1]);
+                    const u64 second = MASS ? upto.mass : upto.count, one = second - (MASS ? e[1].mass : e[1].count);
+                    const u64 none = one - (MASS ? e[0].mass : e[0].count);
+                    if (none < target && target <= one) found = true, w[0] = sh.sorted[2 * tid];
+                    else if (one < target && target <= second) found = true, w[0] = sh.sorted[2 * tid + 1];
+                }
+                tell(found, w, got);
+                return max(cut, got[0]);
+            }
+            // too many for the list: the range of their keys, halved, quartered, .. into buckets again
+            unsigned lo = ~0u, hi = 0;
+            for (int i = tid; i < n; i += S_THREADS) {
+                const unsigned k = key(i);
+                if (k <= KEY_NEG_INF || order_of(k, first + i) < cut || (level && (k < k_lo || k > k_hi)) || bucket(k) != crossing) continue;
+                lo = min(lo, k), hi = max(hi, k);
+            }
+            for (int o = 16; o; o >>= 1) {
+                lo = min(lo, __shfl_xor_sync(~0u, lo, o));
+                hi = max(hi, __shfl_xor_sync(~0u, hi, o));
+            }
+            __syncthreads();
+            if (lane == 0) sh.part[warp] = {lo, hi};
+            __syncthreads();
+            if (tid == 0) {
+                for (int j = 1; j < S_WARPS; j++) lo = min(lo, (unsigned)sh.part[j].count), hi = max(hi, (unsigned)sh.part[j].mass);
+                sh.part[S_WARPS] = {lo, hi};
+            }
+            __syncthreads();
+            if (tid < ranks) cl.map_shared_rank(&sh, tid)->all[turn][rank] = sh.part[S_WARPS];
+            cl.sync();
+            lo = ~0u, hi = 0;
+            for (int r = 0; r < ranks; r++) lo = min(lo, (unsigned)sh.all[turn][r].count), hi = max(hi, (unsigned)sh.all[turn][r].mass);
+            turn ^= 1;
+            if (lo == hi) {  // equal ones: so many, by index
+                const u64 each = MASS ? weight.mass(lo) : 1, need = (target - (MASS ? done.mass : done.count) + each - 1) / each;
+                u64 total_, at_;
+                const int i = locate([&](int j) -> u64 { return key(j) == lo && order_of(lo, first + j) >= cut; },
+                                     [&](u64) { return need - 1; }, total_, at_);
+                return max(cut, order_of(lo, i));
+            }
+            k_lo = lo, k_hi = hi;
+            for (shift = 0; (k_hi - k_lo) >> shift >= S_BUCKETS;) shift++;
+        }
+    }
+};
+
+template <class T>
+__global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args p, int per) {
+    __shared__ SampleShared sh;
+    extern __shared__ __align__(16) uint8_t dyn[];
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");  // (the CTAs of the row have begun)
+    pdl_wait();
+    T *vals = (T *)dyn;
+    const cg::cluster_group cl = cg::this_cluster();
+    const int ranks = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const int64_t row = blockIdx.x / ranks;
+    const int first = min(rank * per, p.n_vocab), n = min(per, p.n_vocab - first);
+    const T *x = (const T *)p.logits + row * p.row_stride + first;
+    Sampler<T> s{sh, cl, vals, n, first, rank, ranks, tid, warp, lane};
+
+    // the row into shared memory, and its largest entry
     u64 best = 0;
-    for (int i = threadIdx.x; i < n; i += S_THREADS) best = max(best, order_of(key_at(i), i));
-    best = block_max(best, part);
+    constexpr int V = 16 / sizeof(T);
+    const int vec = (uintptr_t)x % 16 == 0 ? n / V : 0;
+    auto take = [&](T v, int i) { best = max(best, order_of(key_of(to_f32(v)), first + i)); };
+    for (int i = tid; i < vec; i += S_THREADS) {
+        struct alignas(16) Vec { T v[V]; } r = ((const Vec *)x)[i];
+        ((Vec *)vals)[i] = r;
+#pragma unroll
+        for (int j = 0; j < V; j++) take(r.v[j], i * V + j);
+    }
+    for (int i = vec * V + tid; i < n; i += S_THREADS) {
+        const T v = x[i];
+        vals[i] = v;
+        take(v, i);
+    }
+    for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
+    if (lane == 0) sh.part[warp].mass = best;
+    __syncthreads();
+    asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
+    if (tid < ranks) {
+        for (int j = 0; j < S_WARPS; j++) best = max(best, sh.part[j].mass);
+        cl.map_shared_rank(&sh, tid)->all[1][rank].mass = best;
+    }
+    cl.sync();
+    best = 0;
+    for (int r = 0; r < ranks; r++) best = max(best, sh.all[1][r].mass);
+
     const unsigned top = (unsigned)(best >> 32);
     const float temp = p.temperature ? p.temperature[row] : 1.0f;
     if (top <= KEY_NEG_INF || !(temp > 0.0f)) {
-        if (threadIdx.x == 0) {
+        if (rank == 0 && tid == 0) {
             p.id[row] = top <= KEY_NEG_INF ? -1 : (int)~(unsigned)best;
             if (p.prob) p.prob[row] = top <= KEY_NEG_INF ? 0.0f : 1.0f;
         }
-        return;
+        return;  // (nobody reads this CTA's shared memory any more)
     }
-    const Weight weight{top, (double)value_of(top), 1.0 / (double)temp};
+    // (an infinite largest logit: the others are infinitely far whatever the temperature)
+    const bool infinite = isinf(value_of(top));
+    const Weight weight{top, (double)value_of(top), infinite ? 1.0 : 1.0 / (double)temp};
     const int k = p.top_k ? p.top_k[row] : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
     double min_w = p.min_p ? (double)p.min_p[row] : 0.0;
     min_w = min_w != min_w ? 0.0 : min(min_w, 1.0);
-
-    // sum over the entries from `bound` on: their number, or their mass
-    auto sum_from = [&](u64 bound, bool masses) {
-        u64 s = 0;
-        for (int i = threadIdx.x; i < n; i += S_THREADS) {
-            const unsigned key = key_at(i);
-            if (key > KEY_NEG_INF && order_of(key, i) >= bound) s += masses ? weight.mass(key) : 1;
-        }
-        return block_sum(s, part);
-    };
-    // the largest bound from which on there is still `want`
-    auto search = [&](u64 want, bool masses) {
-        u64 c = 0;
-        for (int b = 63; b >= 0; b--)
-            if (sum_from(c | 1ull << b, masses) >= want) c |= 1ull << b;
-        return c;
-    };
     u64 cut = 0;
-    if (k > 0 && k < n) cut = search(k, false);
-    if (top_p < 1.0f) {
-        const double want = ceil(max((double)top_p, 0.0) * (double)sum_from(cut, true));
-        cut = max(cut, search(max((u64)want, 1ull), true));
-    }
-    // each thread sums its own run of indexes, so that the running sum goes in index order
-    const int run = (n + S_THREADS - 1) / S_THREADS;
-    const int i0 = min((int)threadIdx.x * run, n), i1 = min(i0 + run, n);
-    auto kept_mass = [&](int i) -> u64 {
-        const unsigned key = key_at(i);
-        if (key <= KEY_NEG_INF || order_of(key, i) < cut) return 0;
-        const double w = weight(key);
-        return w >= min_w ? (u64)__double2ll_rn(w * MASS_ONE) : 0;
-    };
-    u64 mine = 0;
-    for (int i = i0; i < i1; i++) mine += kept_mass(i);
-    const u64 total = block_sum(mine, part);
-    before[threadIdx.x] = mine;
-    __syncthreads();
-    u64 c = 0;
-    for (int t = 0; t < (int)threadIdx.x; t++) c += before[t];
+    if (k > 0 && k < p.n_vocab) cut = s.template find_cut<false>(weight, cut, [&](Sum all) { return min((u64)k, all.count); });
+    if (top_p < 1.0f)
+        cut = s.template find_cut<true>(weight, cut, [&](Sum all) {
+            return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1);
+        });
     const float u = p.u[row];
-    const double at = (u > 0.0f ? (double)u : 0.0) * (double)total;
-    const u64 want = at >= (double)total ? total - 1 : (u64)at;
-    if (want >= c && want < c + mine) {
-        for (int i = i0;; i++) {
-            const u64 m = kept_mass(i);
-            if (want < c + m) {
-                p.id[row] = i;
-                if (p.prob) p.prob[row] = (float)((double)m / (double)total);
-                break;
-            }
-            c += m;
-        }
+    u64 total, mass;
+    const int id = s.locate(
+        [&](int i) -> u64 {
+            const unsigned key = s.key(i);
+            if (key <= KEY_NEG_INF || order_of(key, first + i) < cut) return 0;
+            const double w = weight(key);
+            return w >= min_w ? (u64)__double2ll_rn(w * MASS_ONE) : 0;
+        },
+        [&](u64 all) {
+            const double at = (u > 0.0f ? (double)u : 0.0) * (double)all;
+            return at >= (double)all ? all - 1 : (u64)at;
+        },
+        total, mass);
+    if (rank == 0 && tid == 0) {
+        p.id[row] = id;
+        if (p.prob) p.prob[row] = (float)((double)mass / (double)total);
     }
 }
 
@@ -149,7 +402,7 @@ bool sample_check(const sdy_sample_args *a) {
     const char *bad = nullptr;
     if (!a) bad = "no argument block";
     else if (a->type != T_F32 && a->type != T_F16 && a->type != T_BF16) bad = "type is not F32, F16 or BF16";
-    else if (a->n_row < 0) bad = "bad counts";
+    else if (a->n_row < 0 || a->n_row > 1 << 24) bad = "bad counts";
     else if (a->n_vocab < 1 || a->n_vocab > S_MAX_VOCAB) bad = "n_vocab outside [1, 400000]";
     else if (!strides_fit({a->row_stride})) bad = "negative stride";
     else if (a->n_row && (!a->logits || !a->u || !a->id)) bad = "logits, u or id missing";
@@ -172,11 +425,37 @@ bool sample_check(const sdy_sample_args *a) {
 
 }  // namespace
 
-void sample_rows(const sdy_sample_args &a, cudaStream_t s) {
-    if (a.type == T_F32) launch(sample_kernel<float>, a.n_row, S_THREADS, 0, s, a);
-    else if (a.type == T_F16) launch(sample_kernel<__half>, a.n_row, S_THREADS, 0, s, a);
-    else launch(sample_kernel<__nv_bfloat16>, a.n_row, S_THREADS, 0, s, a);
+// CTAs to a row: as few as hold it (so that no barrier is needed where one does), more while the SMs
+// are not all taken.
+template <class T>
+void sample_launch(const sdy_sample_args &a, cudaStream_t s) {
+    constexpr int64_t ROOM = 198 * 1024;  // beside the static shared memory
+    int ranks = 1;
+    while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 148)) ranks *= 2;
+    const int per = ((a.n_vocab + ranks - 1) / ranks + 15) / 16 * 16;
+    static std::atomic<uint64_t> done{0};
+    smem_limit_once(sample_kernel<T>, (int)ROOM, done);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl_enabled();
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ranks;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.n_row * ranks));
+    cfg.blockDim = dim3(S_THREADS);
+    cfg.dynamicSmemBytes = per * sizeof(T);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SDY_CUDA(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, per));
     SDY_LAUNCHED();
+}
+
+void sample_rows(const sdy_sample_args &a, cudaStream_t s) {
+    if (a.type == T_F32) sample_launch<float>(a, s);
+    else if (a.type == T_F16) sample_launch<__half>(a, s);
+    else sample_launch<__nv_bfloat16>(a, s);
 }
 
 }  // namespace sdy
