@@ -50,15 +50,6 @@ __device__ __forceinline__ float value_of(unsigned key) {
 }
 __device__ __forceinline__ u64 order_of(unsigned key, int i) { return (u64)key << 32 | (unsigned)~i; }
 
-struct Weight {
-    unsigned top;   // key of the largest logit
-    double m, inv;  // its value, 1 / temperature
-    __device__ double operator()(unsigned key) const {
-        return key == top ? 1.0 : exp(((double)value_of(key) - m) * inv);
-    }
-    __device__ u64 mass(unsigned key) const { return (u64)__double2ll_rn((*this)(key) * MASS_ONE); }
-};
-
 struct Sum {
     u64 count, mass;
     __device__ Sum operator+(const Sum &o) const { return {count + o.count, mass + o.mass}; }
@@ -72,23 +63,65 @@ struct SampleShared {
     Sum part[S_WARPS + 1];                                    // per warp, then the CTA
     Sum all[2][S_CLUSTER];                                    // exchanged, by rank; two in turn
     u64 said[2][4];                                           // what one CTA tells the others; two in turn
-    u64 best;
+    double power[64];                                         // 2^(j/64)
+};
+__shared__ SampleShared sh;  // (by name, so that accesses are known to be to shared memory)
+extern __shared__ __align__(16) uint8_t sample_row[];
+
+// w = exp(x), x = (logit - max) / temperature <= 0, by the table method: x = (64 n + j) ln 2 / 64 + r, 2^n
+// 2^(j/64) exp(r), |r| <= ln 2 / 128, with the series of exp(r) to r^5 (the rest is below 2^-54).
+struct Weight {
+    unsigned top;   // key of the largest logit
+    double m, inv;  // its value, 1 / temperature
+    // 2^scale w, and 0 for what rounds to no multiple of 2^-44
+    __device__ __forceinline__ double scaled(unsigned key, int scale) const {
+        const double x = ((double)value_of(key) - m) * inv;
+        if (key == top) return __longlong_as_double((u64)(1023 + scale) << 52);
+        if (!(x > -31.2)) return 0.0;
+        constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
+        const double t = fma(x, 92.332482616893656877, MAGIC);
+        const int k = __double2loint(t);
+        const double kd = t - MAGIC;
+        double r = fma(-kd, 0.010830424696249145, x);  // ln 2 / 64 in two parts
+        r = fma(-kd, 3.6235106466348430e-19, r);
+        double e = fma(r, 1.0 / 120, 1.0 / 24);
+        e = fma(e, r, 1.0 / 6);
+        e = fma(e, r, 0.5);
+        e = fma(e, r, 1.0);
+        e = fma(e, r, 1.0) * sh.power[k & 63];
+        return __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 6) + scale) << 52));
+    }
+    __device__ __forceinline__ static u64 whole(double m) {  // nearest integer, below 2^51
+        return (u64)__double_as_longlong(m + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    }
+    __device__ __forceinline__ u64 mass(unsigned key) const { return whole(scaled(key, 44)); }
 };
 
 template <class T>
 struct Sampler {
-    SampleShared &sh;
+    static constexpr int V = 16 / sizeof(T);  // entries read at once
+    struct alignas(16) Vec {
+        T v[V];
+    };
     cg::cluster_group cl;
-    const T *x;     // this CTA's entries
-    int n, first;   // their number, the index of the first
+    int n, first;   // this CTA's entries (a multiple of V, the end filled up with -inf), the index of the first
     int rank, ranks, tid, warp, lane;
     int turn = 0, told = 0;
 
-    __device__ unsigned key(int i) const { return key_of(to_f32(x[i])); }
+    __device__ __forceinline__ unsigned key(int i) const { return key_of(to_f32(((const T *)sample_row)[i])); }
+    // at(key, index here) for all entries, in any order
+    template <class At> __device__ __forceinline__ void each(At at) const {
+        for (int i = tid; i < n / V; i += S_THREADS) {
+            const Vec x = ((const Vec *)sample_row)[i];
+#pragma unroll
+            for (int j = 0; j < V; j++) at(key_of(to_f32(x.v[j])), i * V + j);
+        }
+    }
 
-    // v summed over the warps of the CTA up to and with this thread's; the CTA's sum in sh.part[S_WARPS].
+    // v summed over the threads of the CTA up to and with this one; the CTA's sum in sh.part[S_WARPS].
     __device__ Sum scan(Sum v) {
         Sum in = v;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const Sum u = shfl_up(in, o);
             if (lane >= o) in = in + u;
@@ -96,21 +129,18 @@ struct Sampler {
         __syncthreads();
         if (lane == 31) sh.part[warp] = in;
         __syncthreads();
-        if (warp == 0) {
-            Sum w = lane < S_WARPS ? sh.part[lane] : Sum{0, 0}, t = w;
-            for (int o = 1; o < S_WARPS; o <<= 1) {
-                const Sum u = shfl_up(t, o);
-                if (lane >= o) t = t + u;
-            }
-            __syncwarp();
-            if (lane < S_WARPS) sh.part[lane] = {t.count - w.count, t.mass - w.mass};
-            if (lane == S_WARPS - 1) sh.part[S_WARPS] = t;
+        Sum below = {0, 0}, total = {0, 0};
+#pragma unroll
+        for (int w = 0; w < S_WARPS; w++) {
+            if (w < warp) below = below + sh.part[w];
+            total = total + sh.part[w];
         }
-        __syncthreads();
-        return sh.part[warp] + in;
+        if (tid == 0) sh.part[S_WARPS] = total;
+        return below + in;
     }
     // The sums of the CTAs of lower rank and of all, from every CTA's sum in sh.part[S_WARPS].
     __device__ void exchange(Sum &before, Sum &total) {
+        __syncthreads();
         if (tid < ranks) cl.map_shared_rank(&sh, tid)->all[turn][rank] = sh.part[S_WARPS];
         cl.sync();
         before = total = {0, 0};
@@ -120,81 +150,112 @@ struct Sampler {
         }
         turn ^= 1;
     }
-    // Four numbers from the one CTA in which one thread's `mine` is set, to all.
+    // Four numbers from the one thread in the cluster whose `mine` is set, to all; its warp stores them.
     __device__ void tell(bool mine, const u64 (&v)[4], u64 (&got)[4]) {
-        if (mine)
-            for (int r = 0; r < ranks; r++)
-                for (int i = 0; i < 4; i++) cl.map_shared_rank(&sh, r)->said[told][i] = v[i];
+        const unsigned who = __ballot_sync(~0u, mine);
+        if (who) {
+            u64 word = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const u64 x = __shfl_sync(~0u, v[i], __ffs(who) - 1);
+                if (lane % 4 == i) word = x;
+            }
+            if (lane / 4 < ranks) cl.map_shared_rank(&sh, lane / 4)->said[told][lane % 4] = word;
+        }
         cl.sync();
+#pragma unroll
         for (int i = 0; i < 4; i++) got[i] = sh.said[told][i];
         told ^= 1;
     }
 
-    // The index at which the running sum of f(i), in index order, passes `want_of(total)`; the sum of
-    // all and the f there in `total` and `at`.
+    // The index at which the running sum of f(key, index), in index order, passes want_of(total); the
+    // sum of all and the f there in `total` and `at`.
     template <class F, class W>
     __device__ int locate(F f, W want_of, u64 &total, u64 &at) {
         // a warp's entries are a run of indexes
-        const int per = (n + S_WARPS * 32 - 1) / (S_WARPS * 32) * 32, i0 = min(warp * per, n), i1 = min(i0 + per, n);
+        const int per = (n / V + S_WARPS - 1) / S_WARPS, i0 = min(warp * per, n / V), i1 = min(i0 + per, n / V);
+        auto vec = [&](int i) -> u64 {
+            u64 sum = 0;
+            if (i < i1) {
+                const Vec x = ((const Vec *)sample_row)[i];
+#pragma unroll
+                for (int j = 0; j < V; j++) sum += f(key_of(to_f32(x.v[j])), i * V + j);
+            }
+            return sum;
+        };
         u64 mine = 0;
-        for (int i = i0 + lane; i < i1; i += 32) mine += f(i);
+        for (int i = i0 + lane; i < i1; i += 32) mine += vec(i);
         for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
         const Sum to = scan({0, lane == 31 ? mine : 0});
         Sum before, sum;
         exchange(before, sum);
         total = sum.mass;
         const u64 want = want_of(total), end = before.mass + __shfl_sync(~0u, to.mass, 31), begin = end - mine;
-        bool mine_it = false;
+        bool here = false;
         u64 v[4] = {0, 0, 0, 0};
         if (want >= begin && want < end) {
             u64 c = begin;
             for (int i = i0;; i += 32) {
-                const u64 m = i + lane < i1 ? f(i + lane) : 0;
+                const u64 m = vec(i + lane);
                 u64 in = m;
+#pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const u64 u = __shfl_up_sync(~0u, in, o);
                     if (lane >= o) in += u;
                 }
                 const unsigned past = __ballot_sync(~0u, want < c + in);
                 if (past) {
-                    mine_it = lane == __ffs(past) - 1;
-                    v[0] = first + i + lane, v[1] = m;
+                    here = lane == __ffs(past) - 1;
+                    if (here) {
+                        c += in - m;
+                        for (int j = (i + lane) * V;; j++) {
+                            const u64 one = f(key(j), j);
+                            if (want < c + one) {
+                                v[0] = first + j, v[1] = one;
+                                break;
+                            }
+                            c += one;
+                        }
+                    }
                     break;
                 }
                 c += __shfl_sync(~0u, in, 31);
             }
+            __syncwarp();
         }
         u64 got[4];
-        tell(mine_it, v, got);
+        tell(here, v, got);
         at = got[1];
         return (int)got[0];
     }
 
     // The lowest order of the shortest prefix whose number (MASS: mass) reaches target_of(the sum of
-    // all entries from `cut` on).
+    // all entries from `cut` on). near: distances can be taken in 32 bits.
     template <bool MASS, class Target>
-    __device__ u64 find_cut(const Weight &weight, u64 cut, Target target_of) {
-        unsigned k_hi = weight.top, k_lo = 0;  // the keys in question (k_lo 0: by distance, else by key)
-        int shift = 0;
-        Sum done = {0, 0};                     // before them
+    __device__ u64 find_cut(const Weight &weight, bool near, u64 cut, Target target_of) {
+        const float top = value_of(weight.top), scale = (float)(weight.inv * S_SCALE);
+        unsigned k_hi = weight.top, k_lo = KEY_NEG_INF + 1;  // the keys in question
+        int shift = -1;                                      // buckets by distance, then by key >> shift
+        Sum done = {0, 0};                                   // before them
         u64 target = 0;
-        for (int level = 0;; level++) {
+        while (true) {
+            auto in_question = [&](unsigned key, int i) { return key >= k_lo && key <= k_hi && order_of(key, first + i) >= cut; };
             auto bucket = [&](unsigned key) -> int {
-                if (level) return (int)((k_hi - key) >> shift);
+                if (shift >= 0) return (int)((k_hi - key) >> shift);
                 if (key == weight.top) return 0;
+                if (near) return (int)fminf((top - value_of(key)) * scale, S_BUCKETS - 1.0f);
                 return (int)fmin((weight.m - (double)value_of(key)) * weight.inv * S_SCALE, S_BUCKETS - 1.0);
             };
             for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
-            unsigned far = 0;  // entries in the last bucket, which has most of them (at level 0 they have no mass)
-            for (int i = tid; i < n; i += S_THREADS) {
-                const unsigned k = key(i);
-                if (k <= KEY_NEG_INF || order_of(k, first + i) < cut || (level && (k < k_lo || k > k_hi))) continue;
+            unsigned far = 0;  // by distance, the last bucket has most entries (and none of them mass)
+            each([&](unsigned k, int i) {
+                if (!in_question(k, i)) return;
                 const int b = bucket(k);
-                if (b == S_BUCKETS - 1 && !level) {
+                if (b == S_BUCKETS - 1 && shift < 0) {
                     far++;
-                    continue;
+                    return;
                 }
                 atomicAdd(&sh.count[b], 1u);
                 if (MASS) {
@@ -203,7 +264,7 @@ struct Sampler {
                     const unsigned high = (unsigned)(m >> 32) + (old + low < low);
                     if (high) atomicAdd(&sh.hi[b], high);
                 }
-            }
+            });
             for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(~0u, far, o);
             if (lane == 0 && far) atomicAdd(&sh.count[S_BUCKETS - 1], far);
             cl.sync();
@@ -215,12 +276,13 @@ struct Sampler {
                 if (j < per && tid * per + j < run)
                     for (int r = 0; r < ranks; r++) {
                         const SampleShared *o = cl.map_shared_rank(&sh, r);
-                        own[j] = own[j] + Sum{o->count[b0 + j], (u64)o->hi[b0 + j] << 32 | o->lo[b0 + j]};
+                        own[j].count += o->count[b0 + j];
+                        if (MASS) own[j].mass += (u64)o->hi[b0 + j] << 32 | o->lo[b0 + j];
                     }
             const Sum to = scan(own[0] + own[1]);
             Sum before, total;
             exchange(before, total);
-            if (!level) target = target_of(total);
+            if (shift < 0) target = target_of(total);
             // the bucket in which the sum reaches the target
             bool here = false;
             u64 v[4] = {0, 0, 0, 0};
@@ -243,12 +305,9 @@ struct Sampler {
             if (got[3] <= S_LIST) {
                 // gathered and ranked in the first CTA: every entry counts the ones before it
                 SampleShared *lead = cl.map_shared_rank(&sh, 0);
-                for (int i = tid; i < n; i += S_THREADS) {
-                    const unsigned k = key(i);
-                    if (k <= KEY_NEG_INF || order_of(k, first + i) < cut || (level && (k < k_lo || k > k_hi)) || bucket(k) != crossing)
-                        continue;
-                    lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(k, first + i);
-                }
+                each([&](unsigned k, int i) {
+                    if (in_question(k, i) && bucket(k) == crossing) lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(k, first + i);
+                });
                 cl.sync();
                 bool found = false;
                 u64 w[4] = {0, 0, 0, 0};
@@ -257,6 +316,7 @@ struct Sampler {
                     for (int i = tid; i < m; i += S_THREADS) {
                         const u64 mine = sh.list[i];
                         int at = 0;
+#pragma unroll 8
                         for (int j = 0; j < m; j++) at += sh.list[j] > mine;
                         sh.sorted[at] = mine;
                     }
@@ -276,13 +336,11 @@ struct Sampler {
                 tell(found, w, got);
                 return max(cut, got[0]);
             }
-            // too many for the list: the range of their keys, halved, quartered, .. into buckets again
+            // too many for the list: the range of their keys into buckets again
             unsigned lo = ~0u, hi = 0;
-            for (int i = tid; i < n; i += S_THREADS) {
-                const unsigned k = key(i);
-                if (k <= KEY_NEG_INF || order_of(k, first + i) < cut || (level && (k < k_lo || k > k_hi)) || bucket(k) != crossing) continue;
-                lo = min(lo, k), hi = max(hi, k);
-            }
+            each([&](unsigned k, int i) {
+                if (in_question(k, i) && bucket(k) == crossing) lo = min(lo, k), hi = max(hi, k);
+            });
             for (int o = 16; o; o >>= 1) {
                 lo = min(lo, __shfl_xor_sync(~0u, lo, o));
                 hi = max(hi, __shfl_xor_sync(~0u, hi, o));
@@ -290,20 +348,18 @@ struct Sampler {
             __syncthreads();
             if (lane == 0) sh.part[warp] = {lo, hi};
             __syncthreads();
-            if (tid == 0) {
-                for (int j = 1; j < S_WARPS; j++) lo = min(lo, (unsigned)sh.part[j].count), hi = max(hi, (unsigned)sh.part[j].mass);
-                sh.part[S_WARPS] = {lo, hi};
+            if (tid < ranks) {
+                for (int j = 0; j < S_WARPS; j++) lo = min(lo, (unsigned)sh.part[j].count), hi = max(hi, (unsigned)sh.part[j].mass);
+                cl.map_shared_rank(&sh, tid)->all[turn][rank] = {lo, hi};
             }
-            __syncthreads();
-            if (tid < ranks) cl.map_shared_rank(&sh, tid)->all[turn][rank] = sh.part[S_WARPS];
             cl.sync();
             lo = ~0u, hi = 0;
             for (int r = 0; r < ranks; r++) lo = min(lo, (unsigned)sh.all[turn][r].count), hi = max(hi, (unsigned)sh.all[turn][r].mass);
             turn ^= 1;
             if (lo == hi) {  // equal ones: so many, by index
-                const u64 each = MASS ? weight.mass(lo) : 1, need = (target - (MASS ? done.mass : done.count) + each - 1) / each;
+                const u64 size = MASS ? weight.mass(lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
                 u64 total_, at_;
-                const int i = locate([&](int j) -> u64 { return key(j) == lo && order_of(lo, first + j) >= cut; },
+                const int i = locate([&](unsigned k, int j) -> u64 { return k == lo && order_of(lo, first + j) >= cut; },
                                      [&](u64) { return need - 1; }, total_, at_);
                 return max(cut, order_of(lo, i));
             }
@@ -315,32 +371,32 @@ struct Sampler {
 
 template <class T>
 __global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args p, int per) {
-    __shared__ SampleShared sh;
-    extern __shared__ __align__(16) uint8_t dyn[];
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");  // (the CTAs of the row have begun)
     pdl_wait();
-    T *vals = (T *)dyn;
     const cg::cluster_group cl = cg::this_cluster();
     const int ranks = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int64_t row = blockIdx.x / ranks;
-    const int first = min(rank * per, p.n_vocab), n = min(per, p.n_vocab - first);
+    constexpr int V = Sampler<T>::V;
+    const int first = min(rank * per, p.n_vocab), n = min(per, p.n_vocab - first), full = (n + V - 1) / V * V;
     const T *x = (const T *)p.logits + row * p.row_stride + first;
-    Sampler<T> s{sh, cl, vals, n, first, rank, ranks, tid, warp, lane};
+    Sampler<T> s{cl, full, first, rank, ranks, tid, warp, lane};
+    if (tid >= S_THREADS - 64) sh.power[tid - (S_THREADS - 64)] = exp2((tid - (S_THREADS - 64)) / 64.0);
 
     // the row into shared memory, and its largest entry
     u64 best = 0;
-    constexpr int V = 16 / sizeof(T);
-    const int vec = (uintptr_t)x % 16 == 0 ? n / V : 0;
     auto take = [&](T v, int i) { best = max(best, order_of(key_of(to_f32(v)), first + i)); };
+    const int vec = (uintptr_t)x % 16 == 0 ? n / V : 0;
+#pragma unroll 4
     for (int i = tid; i < vec; i += S_THREADS) {
-        struct alignas(16) Vec { T v[V]; } r = ((const Vec *)x)[i];
-        ((Vec *)vals)[i] = r;
+        const typename Sampler<T>::Vec r = ((const typename Sampler<T>::Vec *)x)[i];
+        ((typename Sampler<T>::Vec *)sample_row)[i] = r;
 #pragma unroll
         for (int j = 0; j < V; j++) take(r.v[j], i * V + j);
     }
-    for (int i = vec * V + tid; i < n; i += S_THREADS) {
-        const T v = x[i];
-        vals[i] = v;
+#pragma unroll 4
+    for (int i = vec * V + tid; i < full; i += S_THREADS) {
+        const T v = i < n ? x[i] : from_f32<T>(-INFINITY);
+        ((T *)sample_row)[i] = v;
         take(v, i);
     }
     for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
@@ -365,26 +421,31 @@ __global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args
         return;  // (nobody reads this CTA's shared memory any more)
     }
     // (an infinite largest logit: the others are infinitely far whatever the temperature)
-    const bool infinite = isinf(value_of(top));
-    const Weight weight{top, (double)value_of(top), infinite ? 1.0 : 1.0 / (double)temp};
+    const float top_value = value_of(top);
+    const Weight weight{top, (double)top_value, isinf(top_value) ? 1.0 : 1.0 / (double)temp};
+    // where no difference nor quotient that matters leaves the range of 32 bits
+    const bool near = fabsf(top_value) < 1e37f && temp > 1e-30f && temp < 1e30f;
     const int k = p.top_k ? p.top_k[row] : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f;
     double min_w = p.min_p ? (double)p.min_p[row] : 0.0;
     min_w = min_w != min_w ? 0.0 : min(min_w, 1.0);
     u64 cut = 0;
-    if (k > 0 && k < p.n_vocab) cut = s.template find_cut<false>(weight, cut, [&](Sum all) { return min((u64)k, all.count); });
+    if (k > 0 && k < p.n_vocab) cut = s.template find_cut<false>(weight, near, cut, [&](Sum all) { return min((u64)k, all.count); });
     if (top_p < 1.0f)
-        cut = s.template find_cut<true>(weight, cut, [&](Sum all) {
+        cut = s.template find_cut<true>(weight, near, cut, [&](Sum all) {
             return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1);
         });
+    // keys that are too far for min_p (or for any mass) need no exponential
+    float bound = near ? (float)((double)top_value - (min_w > 0.0 ? fmin(31.3, -log(min_w)) : 31.3) * 1.001 * (double)temp) : -INFINITY;
+    bound -= 1e-5f * fabsf(bound);
+    const unsigned low = max(max(key_of(bound), KEY_NEG_INF + 1), (unsigned)(cut >> 32));
     const float u = p.u[row];
     u64 total, mass;
     const int id = s.locate(
-        [&](int i) -> u64 {
-            const unsigned key = s.key(i);
-            if (key <= KEY_NEG_INF || order_of(key, first + i) < cut) return 0;
-            const double w = weight(key);
-            return w >= min_w ? (u64)__double2ll_rn(w * MASS_ONE) : 0;
+        [&](unsigned key, int i) -> u64 {
+            if (key < low || order_of(key, first + i) < cut) return 0;
+            const double w = weight.scaled(key, 44);
+            return w >= min_w * MASS_ONE ? Weight::whole(w) : 0;
         },
         [&](u64 all) {
             const double at = (u > 0.0f ? (double)u : 0.0) * (double)all;
@@ -429,7 +490,7 @@ bool sample_check(const sdy_sample_args *a) {
 // are not all taken.
 template <class T>
 void sample_launch(const sdy_sample_args &a, cudaStream_t s) {
-    constexpr int64_t ROOM = 198 * 1024;  // beside the static shared memory
+    constexpr int64_t ROOM = 197 * 1024;  // beside the static shared memory
     int ranks = 1;
     while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 148)) ranks *= 2;
     const int per = ((a.n_vocab + ranks - 1) / ranks + 15) / 16 * 16;
