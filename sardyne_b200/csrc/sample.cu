@@ -25,6 +25,8 @@
 #include "sardyne_b200.h"
 
 #include <cooperative_groups.h>
+#include <float.h>
+#include <limits.h>
 #include <math.h>
 
 namespace sdy {
@@ -35,20 +37,22 @@ constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32;
 constexpr int S_MAX_VOCAB = SAMPLE_MAX_VOCAB;
 constexpr int S_CLUSTER = 8;                   // CTAs to a row, at most
 constexpr int S_BUCKETS = 1024, S_LIST = 1024;  // the list: entries ranked at once
+constexpr int S_FEW = 256;                     // a top-k that the first CTA finishes alone
 constexpr double S_SCALE = 32.0;               // buckets per unit of (max - l) / T
-constexpr unsigned KEY_NEG_INF = 0x007FFFFFu;  // key(-inf); NaN takes key 0
+constexpr double S_FAR = 31.3;                 // exp(-31.3) 2^44 < 1/2: no mass from here on
 constexpr double MASS_ONE = 17592186044416.0;  // 2^44
 typedef unsigned long long u64;
 
 __device__ __forceinline__ unsigned key_of(float x) {
-    if (x != x) return 0;
-    const unsigned b = __float_as_uint(x + 0.0f);  // (-0 is the same logit as 0)
+    const unsigned b = __float_as_uint(x);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(unsigned key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-__device__ __forceinline__ u64 order_of(unsigned key, int i) { return (u64)key << 32 | (unsigned)~i; }
+__device__ __forceinline__ u64 order_of(float x, int i) { return (u64)key_of(x) << 32 | (unsigned)~i; }
+__device__ __forceinline__ float value_of(u64 order) { return value_of((unsigned)(order >> 32)); }
+__device__ __forceinline__ int index_of(u64 order) { return (int)~(unsigned)order; }
 
 struct Sum {
     u64 count, mass;
@@ -59,42 +63,47 @@ __device__ __forceinline__ Sum shfl_up(Sum v, int o) { return {__shfl_up_sync(~0
 struct SampleShared {
     unsigned count[S_BUCKETS], lo[S_BUCKETS], hi[S_BUCKETS];  // of this CTA's entries (mass in two words)
     u64 list[S_LIST], sorted[S_LIST];                         // first CTA: gathered entries
-    unsigned n_list;
+    unsigned n_list, keep;
     Sum part[S_WARPS + 1];                                    // per warp, then the CTA
     Sum all[2][S_CLUSTER];                                    // exchanged, by rank; two in turn
     u64 said[2][4];                                           // what one CTA tells the others; two in turn
-    double power[64];                                         // 2^(j/64)
+    double power[256];                                        // 2^(j/256)
 };
 __shared__ SampleShared sh;  // (by name, so that accesses are known to be to shared memory)
 extern __shared__ __align__(16) uint8_t sample_row[];
 
-// w = exp(x), x = (logit - max) / temperature <= 0, by the table method: x = (64 n + j) ln 2 / 64 + r, 2^n
-// 2^(j/64) exp(r), |r| <= ln 2 / 128, with the series of exp(r) to r^5 (the rest is below 2^-54).
+// w = exp(x), x = (logit - max) / temperature <= 0, by the table method: y = x 256 / ln 2 = k + f with k
+// whole and |f| <= 1/2, and w = 2^(k/256) 2^(f/256), the second factor by its series to f^4 (the rest is
+// below 2^-53).
 struct Weight {
-    unsigned top;   // key of the largest logit
-    double m, inv;  // its value, 1 / temperature
-    // 2^scale w, and 0 for what rounds to no multiple of 2^-44
-    __device__ __forceinline__ double scaled(unsigned key, int scale) const {
-        const double x = ((double)value_of(key) - m) * inv;
-        if (key == top) return __longlong_as_double((u64)(1023 + scale) << 52);
-        if (!(x > -31.2)) return 0.0;
+    float top;          // the largest logit
+    double m, inv, by;  // the same; 1 / temperature; 256 / (temperature ln 2)
+    // 2^44 w, and 0 for what rounds to no whole number
+    __device__ __forceinline__ double scaled(float v) const {
         constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
-        const double t = fma(x, 92.332482616893656877, MAGIC);
+        constexpr double C = 0.0027076061740622863;   // ln 2 / 256
+        if (v == top) return MASS_ONE;
+        const double d = (double)v - m;
+        if (!(d * inv > -S_FAR)) return 0.0;
+        const double t = fma(d, by, MAGIC), kd = t - MAGIC, f = fma(d, by, -kd);
         const int k = __double2loint(t);
-        const double kd = t - MAGIC;
-        double r = fma(-kd, 0.010830424696249145, x);  // ln 2 / 64 in two parts
-        r = fma(-kd, 3.6235106466348430e-19, r);
-        double e = fma(r, 1.0 / 120, 1.0 / 24);
-        e = fma(e, r, 1.0 / 6);
-        e = fma(e, r, 0.5);
-        e = fma(e, r, 1.0);
-        e = fma(e, r, 1.0) * sh.power[k & 63];
-        return __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 6) + scale) << 52));
+        double e = fma(f, C * C * C * C / 24, C * C * C / 6);
+        e = fma(e, f, C * C / 2);
+        e = fma(e, f, C);
+        e = fma(e, f, 1.0) * sh.power[k & 255];
+        return __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 8) + 44) << 52));
     }
     __device__ __forceinline__ static u64 whole(double m) {  // nearest integer, below 2^51
         return (u64)__double_as_longlong(m + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
     }
-    __device__ __forceinline__ u64 mass(unsigned key) const { return whole(scaled(key, 44)); }
+    __device__ __forceinline__ u64 mass(float v) const { return whole(scaled(v)); }
+};
+
+// The entries from one on, in their order.
+struct Cut {
+    float value;
+    int index;
+    __device__ __forceinline__ bool keeps(float v, int i) const { return v > value || (v == value && i <= index); }
 };
 
 template <class T>
@@ -106,16 +115,25 @@ struct Sampler {
     cg::cluster_group cl;
     int n, first;   // this CTA's entries (a multiple of V, the end filled up with -inf), the index of the first
     int rank, ranks, tid, warp, lane;
+    Weight weight;
+    bool near;      // distances can be taken in 32 bits
+    float scale;    // buckets per unit of logit
     int turn = 0, told = 0;
 
-    __device__ __forceinline__ unsigned key(int i) const { return key_of(to_f32(((const T *)sample_row)[i])); }
-    // at(key, index here) for all entries, in any order
+    // at(value, index here) for all entries, in any order
     template <class At> __device__ __forceinline__ void each(At at) const {
+#pragma unroll 2
         for (int i = tid; i < n / V; i += S_THREADS) {
             const Vec x = ((const Vec *)sample_row)[i];
 #pragma unroll
-            for (int j = 0; j < V; j++) at(key_of(to_f32(x.v[j])), i * V + j);
+            for (int j = 0; j < V; j++) at(to_f32(x.v[j]), i * V + j);
         }
+    }
+    // Buckets by distance from the largest; the last one's entries have no mass.
+    __device__ __forceinline__ int bucket(float v) const {
+        if (v == weight.top) return 0;
+        const float x = near ? (weight.top - v) * scale : (float)fmin((weight.m - (double)v) * weight.inv * S_SCALE, 1e6);
+        return (int)(__float_as_uint(fminf(x, S_BUCKETS - 1.0f) + 8388608.0f) & (S_BUCKETS - 1));
     }
 
     // v summed over the threads of the CTA up to and with this one; the CTA's sum in sh.part[S_WARPS].
@@ -138,17 +156,22 @@ struct Sampler {
         if (tid == 0) sh.part[S_WARPS] = total;
         return below + in;
     }
-    // The sums of the CTAs of lower rank and of all, from every CTA's sum in sh.part[S_WARPS].
-    __device__ void exchange(Sum &before, Sum &total) {
+    // One Sum of every CTA, sh.part[S_WARPS], to all: in sh.all[the result].
+    __device__ int gather_sums() {
         __syncthreads();
         if (tid < ranks) cl.map_shared_rank(&sh, tid)->all[turn][rank] = sh.part[S_WARPS];
         cl.sync();
+        turn ^= 1;
+        return turn ^ 1;
+    }
+    // The sums of the CTAs of lower rank and of all.
+    __device__ void exchange(Sum &before, Sum &total) {
+        const int at = gather_sums();
         before = total = {0, 0};
         for (int r = 0; r < ranks; r++) {
-            if (r < rank) before = before + sh.all[turn][r];
-            total = total + sh.all[turn][r];
+            if (r < rank) before = before + sh.all[at][r];
+            total = total + sh.all[at][r];
         }
-        turn ^= 1;
     }
     // Four numbers from the one thread in the cluster whose `mine` is set, to all; its warp stores them.
     __device__ void tell(bool mine, const u64 (&v)[4], u64 (&got)[4]) {
@@ -167,25 +190,43 @@ struct Sampler {
         for (int i = 0; i < 4; i++) got[i] = sh.said[told][i];
         told ^= 1;
     }
+    // Ranks the first CTA's list of m entries: every one counts the ones before it.
+    __device__ void rank_list(int m) {
+        for (int i = tid; i < m; i += S_THREADS) {
+            const u64 mine = sh.list[i];
+            int at = 0;
+#pragma unroll 8
+            for (int j = 0; j < m; j++) at += sh.list[j] > mine;
+            sh.sorted[at] = mine;
+        }
+        __syncthreads();
+    }
 
-    // The index at which the running sum of f(key, index), in index order, passes want_of(total); the
-    // sum of all and the f there in `total` and `at`.
+    // The index at which the running sum of f(value, index here), in index order, passes
+    // want_of(total); the sum of all and the f there in `total` and `at`.
     template <class F, class W>
     __device__ int locate(F f, W want_of, u64 &total, u64 &at) {
-        // a warp's entries are a run of indexes
+        // a warp's entries are a run of indexes, in steps of 32 reads, whose sums it notes
+        u64 *steps = sh.sorted + warp * 32;
         const int per = (n / V + S_WARPS - 1) / S_WARPS, i0 = min(warp * per, n / V), i1 = min(i0 + per, n / V);
         auto vec = [&](int i) -> u64 {
             u64 sum = 0;
             if (i < i1) {
                 const Vec x = ((const Vec *)sample_row)[i];
 #pragma unroll
-                for (int j = 0; j < V; j++) sum += f(key_of(to_f32(x.v[j])), i * V + j);
+                for (int j = 0; j < V; j++) sum += f(to_f32(x.v[j]), i * V + j);
             }
             return sum;
         };
+        __syncthreads();  // (sh.sorted has been read)
         u64 mine = 0;
-        for (int i = i0 + lane; i < i1; i += 32) mine += vec(i);
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
+        for (int i = i0, k = 0; i < i1; i += 32, k++) {
+            u64 m = vec(i + lane);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(~0u, m, o);
+            mine += m;
+            if (lane == 0) steps[k] = m;
+        }
         const Sum to = scan({0, lane == 31 ? mine : 0});
         Sum before, sum;
         exchange(before, sum);
@@ -194,32 +235,31 @@ struct Sampler {
         bool here = false;
         u64 v[4] = {0, 0, 0, 0};
         if (want >= begin && want < end) {
-            u64 c = begin;
-            for (int i = i0;; i += 32) {
-                const u64 m = vec(i + lane);
-                u64 in = m;
+            auto prefix = [&](u64 m) {
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const u64 u = __shfl_up_sync(~0u, in, o);
-                    if (lane >= o) in += u;
+                    const u64 u = __shfl_up_sync(~0u, m, o);
+                    if (lane >= o) m += u;
                 }
-                const unsigned past = __ballot_sync(~0u, want < c + in);
-                if (past) {
-                    here = lane == __ffs(past) - 1;
-                    if (here) {
-                        c += in - m;
-                        for (int j = (i + lane) * V;; j++) {
-                            const u64 one = f(key(j), j);
-                            if (want < c + one) {
-                                v[0] = first + j, v[1] = one;
-                                break;
-                            }
-                            c += one;
-                        }
+                return m;
+            };
+            // the step, the read, the entry
+            const u64 step = lane * 32 < i1 - i0 ? steps[lane] : 0, upto = prefix(step);
+            const int k = __ffs(__ballot_sync(~0u, want < begin + upto)) - 1;
+            u64 c = begin + __shfl_sync(~0u, upto - step, k);
+            const int i = i0 + 32 * k + lane;
+            const u64 m = vec(i), in = prefix(m);
+            here = lane == __ffs(__ballot_sync(~0u, want < c + in)) - 1;
+            if (here) {
+                c += in - m;
+                for (int j = i * V;; j++) {
+                    const u64 one = f(to_f32(((const T *)sample_row)[j]), j);
+                    if (want < c + one) {
+                        v[0] = first + j, v[1] = one;
+                        break;
                     }
-                    break;
+                    c += one;
                 }
-                c += __shfl_sync(~0u, in, 31);
             }
             __syncwarp();
         }
@@ -229,37 +269,32 @@ struct Sampler {
         return (int)got[0];
     }
 
-    // The lowest order of the shortest prefix whose number (MASS: mass) reaches target_of(the sum of
-    // all entries from `cut` on). near: distances can be taken in 32 bits.
+    // The shortest prefix of the entries that `cut` keeps whose number (MASS: mass) reaches
+    // target_of(the sum of all of them).
     template <bool MASS, class Target>
-    __device__ u64 find_cut(const Weight &weight, bool near, u64 cut, Target target_of) {
-        const float top = value_of(weight.top), scale = (float)(weight.inv * S_SCALE);
-        unsigned k_hi = weight.top, k_lo = KEY_NEG_INF + 1;  // the keys in question
-        int shift = -1;                                      // buckets by distance, then by key >> shift
-        Sum done = {0, 0};                                   // before them
+    __device__ Cut find_cut(Cut cut, Target target_of) {
+        float v_hi = weight.top, v_lo = -FLT_MAX;  // the values in question
+        unsigned k_hi = 0;                         // key of v_hi, and buckets by key >> shift from it
+        int shift = -1;                            // (at first, buckets by distance)
+        Sum done = {0, 0};                         // before them
         u64 target = 0;
         while (true) {
-            auto in_question = [&](unsigned key, int i) { return key >= k_lo && key <= k_hi && order_of(key, first + i) >= cut; };
-            auto bucket = [&](unsigned key) -> int {
-                if (shift >= 0) return (int)((k_hi - key) >> shift);
-                if (key == weight.top) return 0;
-                if (near) return (int)fminf((top - value_of(key)) * scale, S_BUCKETS - 1.0f);
-                return (int)fmin((weight.m - (double)value_of(key)) * weight.inv * S_SCALE, S_BUCKETS - 1.0);
-            };
+            auto in_question = [&](float v, int i) { return v >= v_lo && v <= v_hi && cut.keeps(v, first + i); };
+            auto place = [&](float v) { return shift < 0 ? bucket(v) : (int)((k_hi - key_of(v)) >> shift); };
             for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
             unsigned far = 0;  // by distance, the last bucket has most entries (and none of them mass)
-            each([&](unsigned k, int i) {
-                if (!in_question(k, i)) return;
-                const int b = bucket(k);
+            each([&](float v, int i) {
+                if (!in_question(v, i)) return;
+                const int b = place(v);
                 if (b == S_BUCKETS - 1 && shift < 0) {
                     far++;
                     return;
                 }
                 atomicAdd(&sh.count[b], 1u);
                 if (MASS) {
-                    const u64 m = weight.mass(k);
+                    const u64 m = weight.mass(v);
                     const unsigned low = (unsigned)m, old = atomicAdd(&sh.lo[b], low);
                     const unsigned high = (unsigned)(m >> 32) + (old + low < low);
                     if (high) atomicAdd(&sh.hi[b], high);
@@ -302,30 +337,22 @@ struct Sampler {
             tell(here, v, got);
             const int crossing = (int)got[0];
             done = {got[1], got[2]};
-            if (got[3] <= S_LIST) {
-                // gathered and ranked in the first CTA: every entry counts the ones before it
+            if (got[3] <= S_LIST) {  // gathered and ranked in the first CTA
                 SampleShared *lead = cl.map_shared_rank(&sh, 0);
-                each([&](unsigned k, int i) {
-                    if (in_question(k, i) && bucket(k) == crossing) lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(k, first + i);
+                each([&](float v, int i) {
+                    if (in_question(v, i) && place(v) == crossing) lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(v, first + i);
                 });
                 cl.sync();
                 bool found = false;
                 u64 w[4] = {0, 0, 0, 0};
                 if (rank == 0) {
                     const int m = (int)got[3];
-                    for (int i = tid; i < m; i += S_THREADS) {
-                        const u64 mine = sh.list[i];
-                        int at = 0;
-#pragma unroll 8
-                        for (int j = 0; j < m; j++) at += sh.list[j] > mine;
-                        sh.sorted[at] = mine;
-                    }
-                    __syncthreads();
+                    rank_list(m);
                     Sum e[2];
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         const int i = 2 * tid + j;
-                        e[j] = i < m ? Sum{1, MASS ? weight.mass((unsigned)(sh.sorted[i] >> 32)) : 0} : Sum{0, 0};
+                        e[j] = i < m ? Sum{1, MASS ? weight.mass(value_of(sh.sorted[i])) : 0} : Sum{0, 0};
                     }
                     const Sum upto = done + scan(e[0] + e[1]);
                     const u64 second = MASS ? upto.mass : upto.count, one = second - (MASS ? e[1].mass : e[1].count);
@@ -334,12 +361,12 @@ struct Sampler {
                     else if (one < target && target <= second) found = true, w[0] = sh.sorted[2 * tid + 1];
                 }
                 tell(found, w, got);
-                return max(cut, got[0]);
+                return {value_of(got[0]), index_of(got[0])};
             }
             // too many for the list: the range of their keys into buckets again
             unsigned lo = ~0u, hi = 0;
-            each([&](unsigned k, int i) {
-                if (in_question(k, i) && bucket(k) == crossing) lo = min(lo, k), hi = max(hi, k);
+            each([&](float v, int i) {
+                if (in_question(v, i) && place(v) == crossing) lo = min(lo, key_of(v)), hi = max(hi, key_of(v));
             });
             for (int o = 16; o; o >>= 1) {
                 lo = min(lo, __shfl_xor_sync(~0u, lo, o));
@@ -348,24 +375,88 @@ struct Sampler {
             __syncthreads();
             if (lane == 0) sh.part[warp] = {lo, hi};
             __syncthreads();
-            if (tid < ranks) {
-                for (int j = 0; j < S_WARPS; j++) lo = min(lo, (unsigned)sh.part[j].count), hi = max(hi, (unsigned)sh.part[j].mass);
-                cl.map_shared_rank(&sh, tid)->all[turn][rank] = {lo, hi};
+            if (tid == 0) {
+                for (int j = 1; j < S_WARPS; j++) lo = min(lo, (unsigned)sh.part[j].count), hi = max(hi, (unsigned)sh.part[j].mass);
+                sh.part[S_WARPS] = {lo, hi};
             }
-            cl.sync();
+            const int at = gather_sums();
             lo = ~0u, hi = 0;
-            for (int r = 0; r < ranks; r++) lo = min(lo, (unsigned)sh.all[turn][r].count), hi = max(hi, (unsigned)sh.all[turn][r].mass);
-            turn ^= 1;
+            for (int r = 0; r < ranks; r++) lo = min(lo, (unsigned)sh.all[at][r].count), hi = max(hi, (unsigned)sh.all[at][r].mass);
+            v_lo = value_of(lo), v_hi = value_of(hi);
             if (lo == hi) {  // equal ones: so many, by index
-                const u64 size = MASS ? weight.mass(lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
+                const u64 size = MASS ? weight.mass(v_lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
                 u64 total_, at_;
-                const int i = locate([&](unsigned k, int j) -> u64 { return k == lo && order_of(lo, first + j) >= cut; },
+                const int i = locate([&](float v, int j) -> u64 { return v == v_lo && cut.keeps(v, first + j); },
                                      [&](u64) { return need - 1; }, total_, at_);
-                return max(cut, order_of(lo, i));
+                return {v_lo, i};
             }
-            k_lo = lo, k_hi = hi;
-            for (shift = 0; (k_hi - k_lo) >> shift >= S_BUCKETS;) shift++;
+            k_hi = hi;
+            for (shift = 0; (hi - lo) >> shift >= S_BUCKETS;) shift++;
         }
+    }
+
+    // A top-k of at most S_FEW, finished in the first CTA. The k-th largest of the maxima of this CTA's
+    // threads (`largest`) bounds the k-th entry from below, so what is not below the best of the CTAs'
+    // bounds is gathered, and the rest is work on a short list. False, in all CTAs, where the list
+    // would be too long; true with the token in `id` (first CTA, one thread; else -1).
+    __device__ bool few(float largest, int k, float top_p, double min_w, float u, int &id, float &prob) {
+        for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = 0;
+        if (tid == 0) sh.n_list = 0, sh.keep = S_BUCKETS - 1;
+        __syncthreads();
+        if (largest > -INFINITY) atomicAdd(&sh.count[bucket(largest)], 1u);
+        __syncthreads();
+        const unsigned a = sh.count[2 * tid], b = sh.count[2 * tid + 1];
+        const int to = (int)scan({a + b, 0}).count;
+        if (to - (int)(a + b) < k && to >= k) sh.keep = 2 * tid + (to - (int)b < k);
+        __syncthreads();
+        if (tid == 0) sh.part[S_WARPS].count = sh.keep;
+        const int at = gather_sums();
+        int bound = S_BUCKETS - 1;
+        for (int r = 0; r < ranks; r++) bound = min(bound, (int)sh.all[at][r].count);
+        SampleShared *lead = cl.map_shared_rank(&sh, 0);
+        each([&](float v, int i) {
+            if (v > -INFINITY && bucket(v) <= bound) {
+                const unsigned at = atomicAdd(&lead->n_list, 1u);
+                if (at < S_LIST) lead->list[at] = order_of(v, first + i);
+            }
+        });
+        cl.sync();
+        const int m = (int)lead->n_list;
+        cl.sync();  // (read by all: the first CTA may write it again, or leave)
+        if (m > S_LIST) return false;
+        id = -1;
+        if (rank) return true;
+        rank_list(m);
+        // number of entries kept, of the masses in descending order
+        const int kept_k = min(k, m);
+        const double w = tid < kept_k ? weight.scaled(value_of(sh.sorted[tid])) : 0.0;
+        const u64 mass = Weight::whole(w);
+        if (tid == 0) sh.keep = kept_k;
+        const u64 upto = scan({0, mass}).mass;
+        __syncthreads();
+        const u64 all = sh.part[S_WARPS].mass;
+        if (top_p < 1.0f) {
+            const u64 target = max((u64)ceil(max((double)top_p, 0.0) * (double)all), (u64)1);
+            if (upto - mass < target && target <= upto) atomicMin(&sh.keep, (unsigned)tid + 1);
+        }
+        if (tid > 0 && tid < kept_k && w < min_w * MASS_ONE) atomicMin(&sh.keep, (unsigned)tid);
+        __syncthreads();
+        const int keep = (int)sh.keep;
+        if (tid == keep - 1) sh.part[S_WARPS].mass = upto;
+        u64 *masses = sh.list;
+        if (tid < keep) masses[tid] = mass;
+        __syncthreads();
+        const u64 total = sh.part[S_WARPS].mass;
+        const double at_u = (u > 0.0f ? (double)u : 0.0) * (double)total;
+        const u64 want = at_u >= (double)total ? total - 1 : (u64)at_u;
+        if (tid < keep) {
+            const u64 mine = sh.sorted[tid];
+            u64 below = 0;
+#pragma unroll 8
+            for (int j = 0; j < keep; j++) below += (unsigned)sh.sorted[j] > (unsigned)mine ? masses[j] : 0;  // (~index)
+            if (below <= want && want < below + mass) id = index_of(mine), prob = (float)((double)mass / (double)total);
+        }
+        return true;
     }
 };
 
@@ -373,32 +464,35 @@ template <class T>
 __global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args p, int per) {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");  // (the CTAs of the row have begun)
     pdl_wait();
+    using S = Sampler<T>;
     const cg::cluster_group cl = cg::this_cluster();
     const int ranks = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const int64_t row = blockIdx.x / ranks;
-    constexpr int V = Sampler<T>::V;
+    constexpr int V = S::V;
     const int first = min(rank * per, p.n_vocab), n = min(per, p.n_vocab - first), full = (n + V - 1) / V * V;
     const T *x = (const T *)p.logits + row * p.row_stride + first;
-    Sampler<T> s{cl, full, first, rank, ranks, tid, warp, lane};
-    if (tid >= S_THREADS - 64) sh.power[tid - (S_THREADS - 64)] = exp2((tid - (S_THREADS - 64)) / 64.0);
+    if (tid < 256) sh.power[tid] = exp2(tid / 256.0);
 
-    // the row into shared memory, and its largest entry
-    u64 best = 0;
-    auto take = [&](T v, int i) { best = max(best, order_of(key_of(to_f32(v)), first + i)); };
+    // The row into shared memory (NaN as -inf, -0 as 0), and its largest entry: each thread meets its
+    // own in rising order, so the first of equal ones stays.
+    float largest = -INFINITY;
+    int where = 0;
+    auto take = [&](T t, int i) {
+        const float v = to_f32(t) + 0.0f;
+        if (v > largest) largest = v, where = i;
+        return from_f32<T>(v != v ? -INFINITY : v);
+    };
     const int vec = (uintptr_t)x % 16 == 0 ? n / V : 0;
 #pragma unroll 4
     for (int i = tid; i < vec; i += S_THREADS) {
-        const typename Sampler<T>::Vec r = ((const typename Sampler<T>::Vec *)x)[i];
-        ((typename Sampler<T>::Vec *)sample_row)[i] = r;
+        typename S::Vec r = ((const typename S::Vec *)x)[i];
 #pragma unroll
-        for (int j = 0; j < V; j++) take(r.v[j], i * V + j);
+        for (int j = 0; j < V; j++) r.v[j] = take(r.v[j], i * V + j);
+        ((typename S::Vec *)sample_row)[i] = r;
     }
 #pragma unroll 4
-    for (int i = vec * V + tid; i < full; i += S_THREADS) {
-        const T v = i < n ? x[i] : from_f32<T>(-INFINITY);
-        ((T *)sample_row)[i] = v;
-        take(v, i);
-    }
+    for (int i = vec * V + tid; i < full; i += S_THREADS) ((T *)sample_row)[i] = take(i < n ? x[i] : from_f32<T>(-INFINITY), i);
+    u64 best = order_of(largest, first + where);
     for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
     if (lane == 0) sh.part[warp].mass = best;
     __syncthreads();
@@ -411,40 +505,48 @@ __global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args
     best = 0;
     for (int r = 0; r < ranks; r++) best = max(best, sh.all[1][r].mass);
 
-    const unsigned top = (unsigned)(best >> 32);
+    const float top = value_of(best);
     const float temp = p.temperature ? p.temperature[row] : 1.0f;
-    if (top <= KEY_NEG_INF || !(temp > 0.0f)) {
+    if (top == -INFINITY || !(temp > 0.0f)) {
         if (rank == 0 && tid == 0) {
-            p.id[row] = top <= KEY_NEG_INF ? -1 : (int)~(unsigned)best;
-            if (p.prob) p.prob[row] = top <= KEY_NEG_INF ? 0.0f : 1.0f;
+            p.id[row] = top == -INFINITY ? -1 : index_of(best);
+            if (p.prob) p.prob[row] = top == -INFINITY ? 0.0f : 1.0f;
         }
         return;  // (nobody reads this CTA's shared memory any more)
     }
     // (an infinite largest logit: the others are infinitely far whatever the temperature)
-    const float top_value = value_of(top);
-    const Weight weight{top, (double)top_value, isinf(top_value) ? 1.0 : 1.0 / (double)temp};
+    const double inv = isinf(top) ? 1.0 : 1.0 / (double)temp;
+    const Weight weight{top, (double)top, inv, inv * 369.32993046757463};  // 256 / ln 2
     // where no difference nor quotient that matters leaves the range of 32 bits
-    const bool near = fabsf(top_value) < 1e37f && temp > 1e-30f && temp < 1e30f;
+    const bool near = fabsf(top) < 1e37f && temp > 1e-30f && temp < 1e30f;
+    S s{cl, full, first, rank, ranks, tid, warp, lane, weight, near, (float)(inv * S_SCALE)};
     const int k = p.top_k ? p.top_k[row] : 0;
-    const float top_p = p.top_p ? p.top_p[row] : 1.0f;
+    const float top_p = p.top_p ? p.top_p[row] : 1.0f, u = p.u[row];
     double min_w = p.min_p ? (double)p.min_p[row] : 0.0;
     min_w = min_w != min_w ? 0.0 : min(min_w, 1.0);
-    u64 cut = 0;
-    if (k > 0 && k < p.n_vocab) cut = s.template find_cut<false>(weight, near, cut, [&](Sum all) { return min((u64)k, all.count); });
+    int id;
+    if (k > 0 && k <= S_FEW && k < p.n_vocab) {
+        float prob;
+        if (s.few(largest, k, top_p, min_w, u, id, prob)) {
+            if (id >= 0) {
+                p.id[row] = id;
+                if (p.prob) p.prob[row] = prob;
+            }
+            return;
+        }
+    }
+    Cut cut = {-FLT_MAX, INT_MAX};  // every finite entry and +inf
+    if (k > 0 && k < p.n_vocab) cut = s.template find_cut<false>(cut, [&](Sum all) { return min((u64)k, all.count); });
     if (top_p < 1.0f)
-        cut = s.template find_cut<true>(weight, near, cut, [&](Sum all) {
-            return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1);
-        });
-    // keys that are too far for min_p (or for any mass) need no exponential
-    float bound = near ? (float)((double)top_value - (min_w > 0.0 ? fmin(31.3, -log(min_w)) : 31.3) * 1.001 * (double)temp) : -INFINITY;
-    bound -= 1e-5f * fabsf(bound);
-    const unsigned low = max(max(key_of(bound), KEY_NEG_INF + 1), (unsigned)(cut >> 32));
-    const float u = p.u[row];
+        cut = s.template find_cut<true>(cut, [&](Sum all) { return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1); });
+    // what is too far for min_p (or for any mass) needs no exponential
+    float low = near ? (float)((double)top - (min_w > 0.0 ? fmin(S_FAR, -log(min_w)) : S_FAR) * 1.001 * (double)temp) : -FLT_MAX;
+    low = fmaxf(low - 1e-5f * fabsf(low), cut.value);
     u64 total, mass;
-    const int id = s.locate(
-        [&](unsigned key, int i) -> u64 {
-            if (key < low || order_of(key, first + i) < cut) return 0;
-            const double w = weight.scaled(key, 44);
+    id = s.locate(
+        [&](float v, int i) -> u64 {
+            if (!(v >= low) || !cut.keeps(v, first + i)) return 0;
+            const double w = weight.scaled(v);
             return w >= min_w * MASS_ONE ? Weight::whole(w) : 0;
         },
         [&](u64 all) {
@@ -486,13 +588,12 @@ bool sample_check(const sdy_sample_args *a) {
 
 }  // namespace
 
-// CTAs to a row: as few as hold it (so that no barrier is needed where one does), more while the SMs
-// are not all taken.
+// CTAs to a row: as few as hold it, more while that leaves four to an SM.
 template <class T>
 void sample_launch(const sdy_sample_args &a, cudaStream_t s) {
-    constexpr int64_t ROOM = 197 * 1024;  // beside the static shared memory
+    constexpr int64_t ROOM = 196 * 1024;  // beside the static shared memory
     int ranks = 1;
-    while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 148)) ranks *= 2;
+    while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 4 * 148)) ranks *= 2;
     const int per = ((a.n_vocab + ranks - 1) / ranks + 15) / 16 * 16;
     static std::atomic<uint64_t> done{0};
     smem_limit_once(sample_kernel<T>, (int)ROOM, done);
