@@ -588,12 +588,12 @@ bool sample_check(const sdy_sample_args *a) {
 
 }  // namespace
 
-// CTAs to a row: as few as hold it, more while that leaves four to an SM.
+// CTAs to a row: as few as hold it, more while that leaves eight to an SM.
 template <class T>
 void sample_launch(const sdy_sample_args &a, cudaStream_t s) {
     constexpr int64_t ROOM = 196 * 1024;  // beside the static shared memory
     int ranks = 1;
-    while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 4 * 148)) ranks *= 2;
+    while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 8 * 148)) ranks *= 2;
     const int per = ((a.n_vocab + ranks - 1) / ranks + 15) / 16 * 16;
     static std::atomic<uint64_t> done{0};
     smem_limit_once(sample_kernel<T>, (int)ROOM, done);

@@ -1,86 +1,266 @@
-// Attention of drafted tokens over a KV cache (sdy_tree_attention_dev).
+// Attention of drafted tokens over a KV cache (sdy_tree_attention_dev): the checks, the kernel in 32
+// bits, and the one that joins partial results.
 //
 // Sequence s has n_past cached keys, which every live node sees, and n_node drafted ones behind
-// them, of which node i sees its own path to the root. Which those are is one bit per node:
-// the path of i is the path of parent[i] and i itself.
+// them, of which node i sees its own path to the root.
 #include "tree_attention.cuh"
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace sdy {
 namespace {
 
-constexpr int TA_WORDS = TA_MAX_NODES / 32;
-
-// Bits of the nodes on node i's path (itself included) into path[0..n_words); none for a padding
-// node.
-__device__ __forceinline__ void node_path(const int32_t *parent, int i, int n_words, uint32_t *path) {
-    for (int w = 0; w < n_words; w++) path[w] = 0;
-    int j = i;
-    for (; j >= 0; j = node_up(parent, j)) path[j >> 5] |= 1u << (j & 31);
-    if (j == -2)
-        for (int w = 0; w < n_words; w++) path[w] = 0;
+// In 32 bits on the CUDA cores: f32 caches, and 16-bit ones that tree_attention_tc.cu does not take. A
+// CTA holds 16 x RPT rows of one KV head; half-warp y has rows y RPT .., its lane x the keys x, x + 16, ..
+// of a tile of 64 and the elements 4 x .. + 3, 64 + 4 x .., .. of the result, so scores, probabilities
+// and sums of a row stay within its half-warp. K and V tiles come by cp.async, the next ones under this
+// one's products.
+//
+// Bound by HBM for few rows, by the 32-bit multiply-adds (2 x 64 x head_dim per row and tile) for many:
+// a thread's RPT x 4 scores take 4 + RPT shared memory reads of 16 bytes per 16 RPT of them.
+constexpr int FK = 64, F_THREADS = 256;
+struct Fp32Layout {
+    int rows, ld, stages;  // row stride of Q, K and V in floats
+    __host__ __device__ int q() const { return 0; }
+    __host__ __device__ int k(int stage) const { return rows * ld + stage * 2 * FK * ld; }
+    __host__ __device__ int v(int stage) const { return k(stage) + FK * ld; }
+    __host__ __device__ int p() const { return rows * ld + stages * 2 * FK * ld; }
+    __host__ __device__ int bytes() const { return (p() + rows * (FK + 4)) * 4; }
+};
+constexpr int F_SMEM = 217 * 1024;  // beside the static shared memory
+inline int fp32_rows(const sdy_tree_attention_args &a) {
+    const int rows = a.n_node * (a.n_head / a.n_kv_head);
+    return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+inline Fp32Layout fp32_layout(const sdy_tree_attention_args &a) {
+    Fp32Layout l = {fp32_rows(a), a.head_dim + 4, 2};
+    if (l.bytes() > F_SMEM) l.stages = 1;
+    return l;
 }
 
-// One CTA per (head, node, sequence): each warp takes every fourth key it sees, lane l holding
-// elements l, l+32, ..; the warps' running maxima and sums are joined at the end.
-constexpr int SIMPLE_WARPS = 4;
-template <class T>
-__global__ void __launch_bounds__(32 * SIMPLE_WARPS) tree_simple_kernel(const sdy_tree_attention_args p) {
-    __shared__ uint32_t path[TA_WORDS];
-    __shared__ float m_w[SIMPLE_WARPS], l_w[SIMPLE_WARPS], o_w[SIMPLE_WARPS][TA_MAX_DIM];
+template <class T> __device__ __forceinline__ float4 load4(const T *p) {
+    return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
+}
+template <> __device__ __forceinline__ float4 load4(const float *p) { return *(const float4 *)p; }
+template <class T> __device__ __forceinline__ void store_quad(T *out, float4 v, float f) {
+    struct alignas(4 * sizeof(T)) Quad { T v[4]; } q;
+    q.v[0] = from_f32<T>(f == 0.0f ? 0.0f : v.x * f), q.v[1] = from_f32<T>(f == 0.0f ? 0.0f : v.y * f);
+    q.v[2] = from_f32<T>(f == 0.0f ? 0.0f : v.z * f), q.v[3] = from_f32<T>(f == 0.0f ? 0.0f : v.w * f);
+    *(Quad *)out = q;
+}
+
+template <class T, int RPT, int NC>
+__global__ void __launch_bounds__(F_THREADS, 1)
+    tree_fp32_kernel(const sdy_tree_attention_args p, const Fp32Layout lay, Cut *cuts, float *part_o, float2 *part_ml) {
+    constexpr int R = 16 * RPT;
+    __shared__ int64_t scan[F_THREADS / 32], found[8];
+    __shared__ int16_t up[TA_MAX_NODES];
+    __shared__ uint32_t path[TA_MAX_NODES][TA_MAX_NODES / 32 + 1];  // the nodes each node sees; 0: padding
+    extern __shared__ __align__(16) float mem[];
     pdl_wait();
-    const int h = blockIdx.x, node = blockIdx.y, s = blockIdx.z, hd = p.head_dim;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int words = (p.n_node + 31) / 32;
-    if (threadIdx.x == 0) node_path(p.parent ? p.parent + (int64_t)s * p.n_node : nullptr, node, words, path);
-    __syncthreads();
-    const int past = max(p.n_past[s], 0);
-    const int keys = (int)min((int64_t)past + node + 1, (int64_t)p.max_seq);
-    const bool live = path[node >> 5] >> (node & 31) & 1;
-    const T *q = (const T *)p.q + s * p.q_seq + node * p.q_node + h * p.q_head;
-    const int64_t base = s * p.cache_seq + h / (p.n_head / p.n_kv_head) * p.cache_head;
-    const T *K = (const T *)p.k_cache + base, *V = (const T *)p.v_cache + base;
-    constexpr int E = TA_MAX_DIM / 32;
-    float qv[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        qv[e] = lane + 32 * e < hd ? to_f32(q[lane + 32 * e]) * p.scale : 0.0f;
-        o[e] = 0.0f;
-    }
-    for (int j = warp; live && j < keys; j += SIMPLE_WARPS) {
-        const int d = j - past;
-        if (d >= 0 && !(path[d >> 5] >> (d & 31) & 1)) continue;
-        float x = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++)
-            if (lane + 32 * e < hd) x += qv[e] * to_f32(K[j * p.cache_row + lane + 32 * e]);
-        for (int b = 16; b; b >>= 1) x += __shfl_xor_sync(~0u, x, b);
-        const float up = fmaxf(m, x);
-        if (up == -INFINITY) continue;
-        const float keep = expf(m - up), w = expf(x - up);
-        m = up;
-        l = l * keep + w;
-#pragma unroll
-        for (int e = 0; e < E; e++)
-            if (lane + 32 * e < hd) o[e] = o[e] * keep + w * to_f32(V[j * p.cache_row + lane + 32 * e]);
-    }
-    if (lane == 0) m_w[warp] = m, l_w[warp] = l;
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        if (lane + 32 * e < hd) o_w[warp][lane + 32 * e] = o[e];
-    __syncthreads();
-    float top = -INFINITY;
-    for (int w = 0; w < SIMPLE_WARPS; w++) top = fmaxf(top, m_w[w]);
-    for (int e = threadIdx.x; e < hd; e += blockDim.x) {
-        float sum = 0.0f, out = 0.0f;
-        for (int w = 0; w < SIMPLE_WARPS; w++) {
-            if (l_w[w] == 0.0f) continue;
-            const float f = expf(m_w[w] - top);
-            sum += f * l_w[w];
-            out += f * o_w[w][e];
+    const int tid = threadIdx.x, x = tid % 16, y = tid / 16, hd = p.head_dim, ld = lay.ld;
+    const int rep = p.n_head / p.n_kv_head, rows = p.n_node * rep, groups = (rows + R - 1) / R, items = p.n_kv_head * groups;
+    find_share<FK, F_THREADS>(p, items, blockIdx.x, scan, found);
+    if (tid == 0) note_cut<FK>(p, items, groups, blockIdx.x, found, cuts);
+    Share<FK> share(p, found, items);
+    Segment g;
+    float *Q = mem + lay.q(), *P = mem + lay.p();
+    const float c = p.scale * 1.4426950408889634f;
+    for (int seg = 0; share.next(g, groups); seg++) {
+        const Lengths len = lengths_of(p, g.s, g.past);
+        const int32_t *parent = p.parent ? p.parent + (int64_t)g.s * p.n_node : nullptr;
+        const T *kc = (const T *)p.k_cache + g.s * p.cache_seq + g.head * p.cache_head;
+        const T *vc = (const T *)p.v_cache + g.s * p.cache_seq + g.head * p.cache_head;
+        const int quads = hd / 4;
+        // a tile into stage `st`; rows that do not exist are zero
+        auto fetch = [&](int tile, int st) {
+            for (int w = tid; w < FK * quads; w += F_THREADS) {
+                const int r = w / quads, e = 4 * (w - r * quads), j = tile * FK + r;
+                float *k = mem + lay.k(st) + r * ld + e, *v = mem + lay.v(st) + r * ld + e;
+                if (j >= len.keys) {
+                    *(float4 *)k = *(float4 *)v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                } else if (std::is_same<T, float>::value) {
+                    const uint32_t kd = (uint32_t)__cvta_generic_to_shared(k), vd = (uint32_t)__cvta_generic_to_shared(v);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(kd), "l"(kc + j * p.cache_row + e) : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(vd), "l"(vc + j * p.cache_row + e) : "memory");
+                } else {
+                    *(float4 *)k = load4(kc + j * p.cache_row + e);
+                    *(float4 *)v = load4(vc + j * p.cache_row + e);
+                }
+            }
+            asm volatile("cp.async.commit_group;\n" ::: "memory");
+        };
+        __syncthreads();  // the segment before has been read
+        const bool edges = g.t1 * FK > len.cached;
+        if (lay.stages == 2) fetch(g.t0, 0);
+        for (int w = tid; w < R * quads; w += F_THREADS) {
+            const int r = w / quads, e = 4 * (w - r * quads), row = g.group * R + r, node = row / rep;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (row < rows) v = load4((const T *)p.q + g.s * p.q_seq + node * p.q_node + (g.head * rep + row - node * rep) * p.q_head + e);
+            *(float4 *)(Q + r * ld + e) = v;
         }
-        ((T *)p.out)[s * p.out_seq + node * p.out_node + h * p.out_head + e] = from_f32<T>(sum > 0.0f ? out / sum : 0.0f);
+        if (edges) {
+            if (tid < 32) load_tree(up, parent, p.n_node);
+            __syncthreads();
+            for (int i = tid; i < p.n_node; i += F_THREADS) {
+#pragma unroll
+                for (int w = 0; w <= TA_MAX_NODES / 32; w++) path[i][w] = 0;
+                const bool live = walk_tree(up, i, [&](int j) { path[i][j >> 5] |= 1u << (j & 31); });
+                if (!live)
+#pragma unroll
+                    for (int w = 0; w <= TA_MAX_NODES / 32; w++) path[i][w] = 0;
+            }
+        }
+        float m[RPT], l[RPT];
+        float4 o[RPT][NC];
+        int node[RPT];
+        bool live[RPT];
+#pragma unroll
+        for (int i = 0; i < RPT; i++) {
+            const int row = g.group * R + y * RPT + i;
+            node[i] = row < rows ? row / rep : -1;
+            live[i] = true;
+            m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NC; j++) o[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        for (int t = g.t0; t < g.t1; t++) {
+            const int st = lay.stages == 2 ? (t - g.t0) & 1 : 0, j0 = t * FK;
+            if (lay.stages == 2) {
+                if (t + 1 < g.t1) {
+                    fetch(t + 1, st ^ 1);
+                    asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+                } else {
+                    asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+                }
+            } else {
+                fetch(t, 0);
+                asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            }
+            __syncthreads();
+            const float *K = mem + lay.k(st);
+            float *V = mem + lay.v(st);
+            // drafted rows: which keys a row sees; V of padding nodes is zero, and NaN or infinities of
+            // others meet only the rows that see them
+            uint64_t sees[RPT];
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < RPT; i++) sees[i] = ~0ull;
+            if (j0 + FK > len.cached) {
+                const int from = min(max(len.cached - j0, 0), FK), d0 = j0 + from - len.past;  // first drafted row of the tile
+                const int drafted = min(len.keys - j0, FK) - from;
+#pragma unroll
+                for (int i = 0; i < RPT; i++) {
+                    const bool here = node[i] >= 0;
+                    live[i] = here && (path[here ? node[i] : 0][(here ? node[i] : 0) >> 5] >> (node[i] & 31) & 1);
+                    uint64_t bits = 0;
+                    if (live[i] && drafted > 0) {  // bits d0 .. of the path
+                        const uint32_t *w = path[node[i]] + (d0 >> 5);
+                        const int words = TA_MAX_NODES / 32 - (d0 >> 5);  // (the last word is zero)
+                        const uint64_t lo = w[0] | (uint64_t)(words > 1 ? w[1] : 0) << 32, hi = words > 2 ? w[2] : 0;
+                        bits = lo >> (d0 & 31) | ((d0 & 31) ? hi << (64 - (d0 & 31)) : 0);
+                        if (drafted < 64) bits &= (1ull << drafted) - 1;
+                    }
+                    sees[i] = !live[i] ? 0 : from == 64 ? ~0ull : ((1ull << from) - 1) | bits << from;
+                }
+                for (int w = tid; w < max(drafted, 0) * quads; w += F_THREADS) {
+                    const int r = w / quads, d = d0 + r;
+                    float4 *v = (float4 *)(V + (from + r) * ld + 4 * (w - r * quads));
+                    if (!(path[d][d >> 5] >> (d & 31) & 1)) *v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    else odd = odd || !isfinite(v->x) || !isfinite(v->y) || !isfinite(v->z) || !isfinite(v->w);
+                }
+                odd = __syncthreads_or(odd);
+            }
+            float s[RPT][4];
+#pragma unroll
+            for (int i = 0; i < RPT; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
+#pragma unroll 4
+            for (int e = 0; e < hd; e += 4) {
+                float4 q[RPT], k[4];
+#pragma unroll
+                for (int i = 0; i < RPT; i++) q[i] = *(const float4 *)(Q + (y * RPT + i) * ld + e);
+#pragma unroll
+                for (int j = 0; j < 4; j++) k[j] = *(const float4 *)(K + (x + 16 * j) * ld + e);
+#pragma unroll
+                for (int i = 0; i < RPT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        s[i][j] += q[i].x * k[j].x + q[i].y * k[j].y + q[i].z * k[j].z + q[i].w * k[j].w;
+            }
+#pragma unroll
+            for (int i = 0; i < RPT; i++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[i][j] = sees[i] >> (x + 16 * j) & 1 ? s[i][j] * c : -INFINITY;
+                    top = fmaxf(top, s[i][j]);
+                }
+#pragma unroll
+                for (int b = 8; b; b >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, b));
+                const float now = fmaxf(m[i], top), off = now == -INFINITY ? 0.0f : now;
+                const float f = exp2f(m[i] - off);  // (0 at first)
+                m[i] = now;
+                l[i] *= f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float w = exp2f(s[i][j] - off);
+                    l[i] += w;
+                    P[(y * RPT + i) * (FK + 4) + x + 16 * j] = w;
+                }
+#pragma unroll
+                for (int j = 0; j < NC; j++) o[i][j].x *= f, o[i][j].y *= f, o[i][j].z *= f, o[i][j].w *= f;
+            }
+            __syncwarp();
+            auto products = [&](auto skip_zero) {
+#pragma unroll 2
+                for (int k = 0; k < FK; k += 4) {
+                    float4 w[RPT];
+#pragma unroll
+                    for (int i = 0; i < RPT; i++) w[i] = *(const float4 *)(P + (y * RPT + i) * (FK + 4) + k);
+#pragma unroll
+                    for (int j = 0; j < NC; j++) {
+                        const int e = 64 * j + 4 * x;
+                        if (e >= hd) continue;
+#pragma unroll
+                        for (int b = 0; b < 4; b++) {
+                            const float4 v = *(const float4 *)(V + (k + b) * ld + e);
+#pragma unroll
+                            for (int i = 0; i < RPT; i++) {
+                                const float a = b == 0 ? w[i].x : b == 1 ? w[i].y : b == 2 ? w[i].z : w[i].w;
+                                if (skip_zero() && a == 0.0f) continue;
+                                o[i][j].x += a * v.x, o[i][j].y += a * v.y, o[i][j].z += a * v.z, o[i][j].w += a * v.w;
+                            }
+                        }
+                    }
+                }
+            };
+            if (odd) products(std::true_type());
+            else products(std::false_type());
+            __syncthreads();  // the tile has been read
+        }
+        const bool whole = g.t0 == 0 && g.t1 == g.tiles;
+        const int64_t slot = 2 * blockIdx.x + (seg > 0);
+#pragma unroll
+        for (int i = 0; i < RPT; i++) {
+#pragma unroll
+            for (int b = 8; b; b >>= 1) l[i] += __shfl_xor_sync(~0u, l[i], b);
+            if (node[i] < 0) continue;
+            const int r = y * RPT + i, row = g.group * R + r;
+            if (!whole && x == 0) part_ml[slot * R + r] = make_float2(m[i], live[i] ? l[i] : -1.0f);
+            T *out = (T *)p.out + g.s * p.out_seq + node[i] * p.out_node + (g.head * rep + row - node[i] * rep) * p.out_head;
+            float *part = part_o + slot * part_stride(R, hd) + (int64_t)r * hd;
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+                const int e = 64 * j + 4 * x;
+                if (e >= hd) continue;
+                if (whole) store_quad(out + e, o[i][j], live[i] && l[i] != 0.0f ? 1.0f / l[i] : 0.0f);
+                else *(float4 *)(part + e) = o[i][j];
+            }
+        }
     }
 }
 
@@ -94,12 +274,6 @@ __global__ void __launch_bounds__(32 * SIMPLE_WARPS) tree_simple_kernel(const sd
 constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 16, JOIN_BLOCKS = 5 * TA_CTAS;
 constexpr int JOIN_FEW = 4;  // so many parts at most are loaded straight into registers
 constexpr int JOIN_RUNS = (TA_CTAS + 31) / 32;  // cuts, or parts, a lane looks at
-template <class T> __device__ __forceinline__ void store_quad(T *out, float4 v, float f) {
-    struct alignas(4 * sizeof(T)) Quad { T v[4]; } q;
-    q.v[0] = from_f32<T>(f == 0.0f ? 0.0f : v.x * f), q.v[1] = from_f32<T>(f == 0.0f ? 0.0f : v.y * f);
-    q.v[2] = from_f32<T>(f == 0.0f ? 0.0f : v.z * f), q.v[3] = from_f32<T>(f == 0.0f ? 0.0f : v.w * f);
-    *(Quad *)out = q;
-}
 template <class T>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
     join_kernel(const sdy_tree_attention_args p, const Cut *__restrict__ cuts, const float *__restrict__ o,
@@ -236,7 +410,7 @@ const char *counts_bad(const sdy_tree_attention_args *a) {
 }
 
 size_t tree_bytes(const sdy_tree_attention_args &a) {
-    return tree_tc_takes(a) ? tree_space(a, tree_tc_rows(a)).bytes : 256;
+    return tree_space(a, tree_tc_takes(a) ? tree_tc_rows(a) : fp32_rows(a)).bytes;
 }
 
 bool tree_check(const sdy_tree_attention_args *a) {
@@ -272,11 +446,29 @@ bool tree_check(const sdy_tree_attention_args *a) {
     return true;
 }
 
+template <class T, int RPT, int NC>
+void fp32_launch(const sdy_tree_attention_args &a, const TreeSpace &sp, cudaStream_t s) {
+    const Fp32Layout lay = fp32_layout(a);
+    static std::atomic<uint64_t> done{0};
+    smem_limit_once(tree_fp32_kernel<T, RPT, NC>, F_SMEM, done);
+    launch(tree_fp32_kernel<T, RPT, NC>, TA_CTAS, F_THREADS, lay.bytes(), s, a, lay, sp.cuts, sp.o, sp.ml);
+    SDY_LAUNCHED();
+}
+template <class T, int RPT>
+void fp32_pick(const sdy_tree_attention_args &a, const TreeSpace &sp, cudaStream_t s) {
+    if (a.head_dim <= 64) fp32_launch<T, RPT, 1>(a, sp, s);
+    else if (a.head_dim <= 128) fp32_launch<T, RPT, 2>(a, sp, s);
+    else fp32_launch<T, RPT, 4>(a, sp, s);
+}
 template <class T>
 void tree_launch(const sdy_tree_attention_args &a, cudaStream_t s) {
     if (tree_tc_takes(a)) return tree_tc(a, s);
-    launch(tree_simple_kernel<T>, dim3(a.n_head, a.n_node, a.n_seq), 32 * SIMPLE_WARPS, 0, s, a);
-    SDY_LAUNCHED();
+    const int rows = fp32_rows(a);
+    const TreeSpace sp = tree_space(a, rows);
+    if (rows == 16) fp32_pick<T, 1>(a, sp, s);
+    else if (rows == 32) fp32_pick<T, 2>(a, sp, s);
+    else fp32_pick<T, 4>(a, sp, s);
+    tree_join(a, sp, rows, s);
 }
 
 }  // namespace
