@@ -7,7 +7,6 @@
 
 #include <algorithm>
 #include <initializer_list>
-#include <vector>
 
 namespace sdy {
 
@@ -16,39 +15,48 @@ inline int value_bytes(int type) { return type == T_F32 ? 4 : 2; }
 // Ordinal of the device that the driver knows `p` to belong to (false: it knows no such memory).
 bool pointer_device(const void *p, int *device);
 
-// True when the kernels of the current device may use `p`: memory of that device, managed memory,
-// or pinned host memory mapped there. A pointer of another device or of pageable host memory would
-// fault in the kernel, so it is refused here.
-// (The driver's one-attribute query answers for memory of the current device in a fraction of the
-// full query's time; a call makes up to nine.)
-inline bool device_pointer(const char *fn, const char *name, const void *p) {
-    int at_device = -1, current = -1;
-    if (pointer_device(p, &at_device) && cudaGetDevice(&current) == cudaSuccess && at_device == current) return true;
-    cudaPointerAttributes at;
-    if (!SDY_CUDA(cudaPointerGetAttributes(&at, p))) return false;
-    int dev = -1;
-    if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeHost && at.devicePointer == p)) return true;
-    if (at.type == cudaMemoryTypeDevice) {
-        if (!SDY_CUDA(cudaGetDevice(&dev))) return false;
-        if (at.device == dev) return true;
+struct Pointer {
+    const char *name;
+    const void *p;
+};
+// True when the kernels of the current device may use every pointer that is set: memory of that
+// device, managed memory, or pinned host memory mapped there. A pointer of another device or of
+// pageable host memory would fault in the kernel, so it is refused here. (The driver's one-attribute
+// query answers for memory of the current device in a tenth of a microsecond, the full query in
+// three times that; a call has up to nine pointers.)
+inline bool device_pointers(const char *fn, std::initializer_list<Pointer> all) {
+    int current = -1;
+    if (!SDY_CUDA(cudaGetDevice(&current))) return false;
+    for (const Pointer &x : all) {
+        int at_device = -1;
+        if (!x.p || (pointer_device(x.p, &at_device) && at_device == current)) continue;
+        cudaPointerAttributes at;
+        if (!SDY_CUDA(cudaPointerGetAttributes(&at, x.p))) return false;
+        if (at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeHost && at.devicePointer == x.p)) continue;
+        set_error("%s: %s is not memory of the current device", fn, x.name);
+        return false;
     }
-    set_error("%s: %s is not memory of the current device", fn, name);
-    return false;
+    return true;
 }
 
 struct Axis {
     int64_t stride, count;
 };
-// True when the elements of an output with these axes above a contiguous run of `inner` elements
-// cannot coincide: each axis steps over all that the smaller ones span.
+// True when the elements of an output with these axes (three at most) above a contiguous run of `inner`
+// elements cannot coincide: each axis steps over all that the smaller ones span.
 inline bool disjoint(std::initializer_list<Axis> axes, int64_t inner) {
-    std::vector<Axis> a(axes);
-    std::sort(a.begin(), a.end(), [](const Axis &x, const Axis &y) { return x.stride < y.stride; });
+    Axis a[3];  // sorted by stride
+    int n = 0;
+    for (const Axis &x : axes) {
+        if (x.count <= 1 || n == 3) continue;
+        int i = n++;
+        for (; i > 0 && a[i - 1].stride > x.stride; i--) a[i] = a[i - 1];
+        a[i] = x;
+    }
     int64_t span = inner;
-    for (const Axis &x : a) {
-        if (x.count <= 1) continue;
-        if (x.stride < span || x.stride > (int64_t)1 << 48) return false;
-        span += x.stride * (x.count - 1);
+    for (int i = 0; i < n; i++) {
+        if (a[i].stride < span || a[i].stride > (int64_t)1 << 48) return false;
+        span += a[i].stride * (a[i].count - 1);
     }
     return true;
 }

@@ -578,12 +578,7 @@ bool sample_check(const sdy_sample_args *a) {
         return false;
     }
     if (!a->n_row) return true;
-    const struct { const char *name; const void *p; } all[] = {
-        {"logits", a->logits}, {"u", a->u}, {"id", a->id}, {"temperature", a->temperature}, {"top_k", a->top_k},
-        {"top_p", a->top_p}, {"min_p", a->min_p}, {"prob", a->prob}};
-    for (const auto &x : all)
-        if (x.p && !device_pointer(fn, x.name, x.p)) return false;
-    return true;
+    return device_pointers(fn, {{"logits", a->logits}, {"u", a->u}, {"id", a->id}, {"temperature", a->temperature}, {"top_k", a->top_k}, {"top_p", a->top_p}, {"min_p", a->min_p}, {"prob", a->prob}});
 }
 
 }  // namespace

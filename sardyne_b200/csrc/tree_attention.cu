@@ -438,12 +438,7 @@ bool tree_check(const sdy_tree_attention_args *a) {
         return false;
     }
     if (!a->n_seq) return true;
-    const struct { const char *name; const void *p; } all[] = {
-        {"q", a->q}, {"k_cache", a->k_cache}, {"v_cache", a->v_cache}, {"n_past", a->n_past}, {"parent", a->parent},
-        {"out", a->out}, {"ws", a->ws}};
-    for (const auto &x : all)
-        if (x.p && !device_pointer(fn, x.name, x.p)) return false;
-    return true;
+    return device_pointers(fn, {{"q", a->q}, {"k_cache", a->k_cache}, {"v_cache", a->v_cache}, {"n_past", a->n_past}, {"parent", a->parent}, {"out", a->out}, {"ws", a->ws}});
 }
 
 template <class T, int RPT, int NC>
