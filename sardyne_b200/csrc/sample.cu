@@ -37,7 +37,7 @@ constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32;
 constexpr int S_MAX_VOCAB = SAMPLE_MAX_VOCAB;
 constexpr int S_CLUSTER = 8;                   // CTAs to a row, at most
 constexpr int S_BUCKETS = 1024, S_LIST = 1024;  // the list: entries ranked at once
-constexpr int S_FEW = 256;                     // a top-k that the first CTA finishes alone
+constexpr int S_FEW = 512;                     // a top-k that the first CTA finishes alone, one entry to a thread
 constexpr double S_SCALE = 32.0;               // buckets per unit of (max - l) / T
 constexpr double S_FAR = 31.3;                 // exp(-31.3) 2^44 < 1/2: no mass from here on
 constexpr double MASS_ONE = 17592186044416.0;  // 2^44
@@ -82,16 +82,15 @@ struct Weight {
     __device__ __forceinline__ double scaled(float v) const {
         constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
         constexpr double C = 0.0027076061740622863;   // ln 2 / 256
-        if (v == top) return MASS_ONE;
         const double d = (double)v - m;
-        if (!(d * inv > -S_FAR)) return 0.0;
         const double t = fma(d, by, MAGIC), kd = t - MAGIC, f = fma(d, by, -kd);
         const int k = __double2loint(t);
         double e = fma(f, C * C * C * C / 24, C * C * C / 6);
         e = fma(e, f, C * C / 2);
         e = fma(e, f, C);
         e = fma(e, f, 1.0) * sh.power[k & 255];
-        return __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 8) + 44) << 52));
+        e = __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 8) + 44) << 52));
+        return v == top ? MASS_ONE : d * inv > -S_FAR ? e : 0.0;  // (no branch: a thread's entries go abreast)
     }
     __device__ __forceinline__ static u64 whole(double m) {  // nearest integer, below 2^51
         return (u64)__double_as_longlong(m + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
@@ -120,20 +119,32 @@ struct Sampler {
     float scale;    // buckets per unit of logit
     int turn = 0, told = 0;
 
-    // at(value, index here) for all entries, in any order
-    template <class At> __device__ __forceinline__ void each(At at) const {
-#pragma unroll 2
-        for (int i = tid; i < n / V; i += S_THREADS) {
-            const Vec x = ((const Vec *)sample_row)[i];
+    // Entries i V .. of this CTA, -inf behind its last.
+    __device__ __forceinline__ void read(int i, int end, float (&v)[V]) const {
+        Vec x;
+        if (i < end) x = ((const Vec *)sample_row)[i];
 #pragma unroll
-            for (int j = 0; j < V; j++) at(to_f32(x.v[j]), i * V + j);
+        for (int j = 0; j < V; j++) v[j] = i < end ? to_f32(x.v[j]) : -INFINITY;
+    }
+    // at(values, index here of the first) for all entries, by whole warps, in any order
+    template <class At> __device__ __forceinline__ void each(At at) const {
+        for (int i = tid; i - lane < n / V; i += S_THREADS) {
+            float v[V];
+            read(i, n / V, v);
+            at(v, i * V);
         }
+    }
+    // The values that can be in bucket b (and a few around): what is outside need not be placed.
+    __device__ __forceinline__ void bucket_range(int b, float &lo, float &hi) const {
+        const float slack = 1e-6f * (fabsf(weight.top) + (b + 1) / scale);
+        lo = near && b < S_BUCKETS - 1 ? weight.top - (b + 0.51f) / scale - slack : -FLT_MAX;
+        hi = near ? weight.top - (b - 0.51f) / scale + slack : INFINITY;
     }
     // Buckets by distance from the largest; the last one's entries have no mass.
     __device__ __forceinline__ int bucket(float v) const {
-        if (v == weight.top) return 0;
         const float x = near ? (weight.top - v) * scale : (float)fmin((weight.m - (double)v) * weight.inv * S_SCALE, 1e6);
-        return (int)(__float_as_uint(fminf(x, S_BUCKETS - 1.0f) + 8388608.0f) & (S_BUCKETS - 1));
+        const int b = (int)(__float_as_uint(fminf(x, S_BUCKETS - 1.0f) + 8388608.0f) & (S_BUCKETS - 1));
+        return v == weight.top ? 0 : b;
     }
 
     // v summed over the threads of the CTA up to and with this one; the CTA's sum in sh.part[S_WARPS].
@@ -190,31 +201,66 @@ struct Sampler {
         for (int i = 0; i < 4; i++) got[i] = sh.said[told][i];
         told ^= 1;
     }
-    // Ranks the first CTA's list of m entries: every one counts the ones before it.
+    // The first CTA's list of m entries in descending order: sorted bitonically, one entry to a thread,
+    // or, where there are more, every one counts the ones before it.
     __device__ void rank_list(int m) {
-        for (int i = tid; i < m; i += S_THREADS) {
-            const u64 mine = sh.list[i];
-            int at = 0;
+        if (m <= S_THREADS) {
+            u64 mine = tid < m ? sh.list[tid] : 0;
+            int size = 2;
+            for (; size / 2 < m; size *= 2)
+                for (int j = size / 2; j; j /= 2) {
+                    u64 other;
+                    if (j < 32) {
+                        other = __shfl_xor_sync(~0u, mine, j);
+                    } else {
+                        __syncthreads();
+                        sh.sorted[tid] = mine;
+                        __syncthreads();
+                        other = sh.sorted[tid ^ j];
+                    }
+                    // descending where the run's bit is clear; the lower one of a pair keeps the larger
+                    const bool larger = ((tid & size) == 0) == ((tid & j) == 0);
+                    mine = larger == (mine > other) ? mine : other;
+                }
+            __syncthreads();
+            sh.sorted[tid] = mine;
+        } else {
+            for (int i = tid; i < m; i += S_THREADS) {
+                const u64 mine = sh.list[i];
+                int at = 0;
 #pragma unroll 8
-            for (int j = 0; j < m; j++) at += sh.list[j] > mine;
-            sh.sorted[at] = mine;
+                for (int j = 0; j < m; j++) at += sh.list[j] > mine;
+                sh.sorted[at] = mine;
+            }
         }
         __syncthreads();
     }
 
-    // The index at which the running sum of f(value, index here), in index order, passes
-    // want_of(total); the sum of all and the f there in `total` and `at`.
-    template <class F, class W>
-    __device__ int locate(F f, W want_of, u64 &total, u64 &at) {
+    // The index at which the running sum of of(value) over the entries in(value, index here), in index
+    // order, passes want_of(total); the sum of all and the one there in `total` and `at`.
+    template <class In, class Of, class W>
+    __device__ int locate(bool sparse, In in, Of of, W want_of, u64 &total, u64 &at) {
         // a warp's entries are a run of indexes, in steps of 32 reads, whose sums it notes
         u64 *steps = sh.sorted + warp * 32;
         const int per = (n / V + S_WARPS - 1) / S_WARPS, i0 = min(warp * per, n / V), i1 = min(i0 + per, n / V);
-        auto vec = [&](int i) -> u64 {
-            u64 sum = 0;
-            if (i < i1) {
-                const Vec x = ((const Vec *)sample_row)[i];
+        auto vec = [&](int i) -> u64 {  // by whole warps
+            float v[V];
+            bool ok[V], any = false;
+            read(i, i1, v);
 #pragma unroll
-                for (int j = 0; j < V; j++) sum += f(to_f32(x.v[j]), i * V + j);
+            for (int j = 0; j < V; j++) ok[j] = in(v[j], i * V + j), any = any || ok[j];
+            u64 sum = 0;
+            if (!__any_sync(~0u, any)) return sum;
+            if (sparse) {  // (few are in: entry by entry)
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    if (ok[j]) sum += of(v[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const u64 m = of(v[j]);
+                    sum += ok[j] ? m : 0;
+                }
             }
             return sum;
         };
@@ -222,8 +268,9 @@ struct Sampler {
         u64 mine = 0;
         for (int i = i0, k = 0; i < i1; i += 32, k++) {
             u64 m = vec(i + lane);
+            if (__any_sync(~0u, m != 0))
 #pragma unroll
-            for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(~0u, m, o);
+                for (int o = 16; o; o >>= 1) m += __shfl_xor_sync(~0u, m, o);
             mine += m;
             if (lane == 0) steps[k] = m;
         }
@@ -248,12 +295,13 @@ struct Sampler {
             const int k = __ffs(__ballot_sync(~0u, want < begin + upto)) - 1;
             u64 c = begin + __shfl_sync(~0u, upto - step, k);
             const int i = i0 + 32 * k + lane;
-            const u64 m = vec(i), in = prefix(m);
-            here = lane == __ffs(__ballot_sync(~0u, want < c + in)) - 1;
+            const u64 m = vec(i), to_here = prefix(m);
+            here = lane == __ffs(__ballot_sync(~0u, want < c + to_here)) - 1;
             if (here) {
-                c += in - m;
+                c += to_here - m;
                 for (int j = i * V;; j++) {
-                    const u64 one = f(to_f32(((const T *)sample_row)[j]), j);
+                    const float x = to_f32(((const T *)sample_row)[j]);
+                    const u64 one = in(x, j) ? of(x) : 0;
                     if (want < c + one) {
                         v[0] = first + j, v[1] = one;
                         break;
@@ -271,9 +319,11 @@ struct Sampler {
 
     // The shortest prefix of the entries that `cut` keeps whose number (MASS: mass) reaches
     // target_of(the sum of all of them).
+    // bound: a value that the result is not below.
     template <bool MASS, class Target>
-    __device__ Cut find_cut(Cut cut, Target target_of) {
-        float v_hi = weight.top, v_lo = -FLT_MAX;  // the values in question
+    __device__ Cut find_cut(Cut cut, float bound, Target target_of) {
+        float v_hi = weight.top, v_lo = fmaxf(cut.value, bound);  // the values in question
+        const bool sparse = cut.value > -FLT_MAX;
         unsigned k_hi = 0;                         // key of v_hi, and buckets by key >> shift from it
         int shift = -1;                            // (at first, buckets by distance)
         Sum done = {0, 0};                         // before them
@@ -285,19 +335,29 @@ struct Sampler {
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
             unsigned far = 0;  // by distance, the last bucket has most entries (and none of them mass)
-            each([&](float v, int i) {
-                if (!in_question(v, i)) return;
-                const int b = place(v);
-                if (b == S_BUCKETS - 1 && shift < 0) {
-                    far++;
-                    return;
+            each([&](const float(&v)[V], int i) {
+                bool ok[V], any = false;
+#pragma unroll
+                for (int j = 0; j < V; j++) ok[j] = in_question(v[j], i + j), any = any || ok[j];
+                if (!__any_sync(~0u, any)) return;
+                int b[V];
+                u64 m[V];
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    b[j] = place(v[j]);
+                    m[j] = MASS && (!sparse || ok[j]) ? weight.mass(v[j]) : 0;
                 }
-                atomicAdd(&sh.count[b], 1u);
-                if (MASS) {
-                    const u64 m = weight.mass(v);
-                    const unsigned low = (unsigned)m, old = atomicAdd(&sh.lo[b], low);
-                    const unsigned high = (unsigned)(m >> 32) + (old + low < low);
-                    if (high) atomicAdd(&sh.hi[b], high);
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const bool last = shift < 0 && b[j] == S_BUCKETS - 1;
+                    far += ok[j] && last;
+                    if (!ok[j] || last) continue;
+                    atomicAdd(&sh.count[b[j]], 1u);
+                    if (MASS) {
+                        const unsigned low = (unsigned)m[j], old = atomicAdd(&sh.lo[b[j]], low);
+                        const unsigned high = (unsigned)(m[j] >> 32) + (old + low < low);
+                        if (high) atomicAdd(&sh.hi[b[j]], high);
+                    }
                 }
             });
             for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(~0u, far, o);
@@ -337,10 +397,16 @@ struct Sampler {
             tell(here, v, got);
             const int crossing = (int)got[0];
             done = {got[1], got[2]};
+            float lo_v = v_lo, hi_v = v_hi;
+            if (shift < 0) bucket_range(crossing, lo_v, hi_v);
+            lo_v = fmaxf(lo_v, v_lo);
+            auto is_crossing = [&](float v, int i) { return v >= lo_v && v <= hi_v && in_question(v, i) && place(v) == crossing; };
             if (got[3] <= S_LIST) {  // gathered and ranked in the first CTA
                 SampleShared *lead = cl.map_shared_rank(&sh, 0);
-                each([&](float v, int i) {
-                    if (in_question(v, i) && place(v) == crossing) lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(v, first + i);
+                each([&](const float(&v)[V], int i) {
+#pragma unroll
+                    for (int j = 0; j < V; j++)
+                        if (is_crossing(v[j], i + j)) lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(v[j], first + i + j);
                 });
                 cl.sync();
                 bool found = false;
@@ -365,8 +431,10 @@ struct Sampler {
             }
             // too many for the list: the range of their keys into buckets again
             unsigned lo = ~0u, hi = 0;
-            each([&](float v, int i) {
-                if (in_question(v, i) && place(v) == crossing) lo = min(lo, key_of(v)), hi = max(hi, key_of(v));
+            each([&](const float(&v)[V], int i) {
+#pragma unroll
+                for (int j = 0; j < V; j++)
+                    if (is_crossing(v[j], i + j)) lo = min(lo, key_of(v[j])), hi = max(hi, key_of(v[j]));
             });
             for (int o = 16; o; o >>= 1) {
                 lo = min(lo, __shfl_xor_sync(~0u, lo, o));
@@ -386,7 +454,7 @@ struct Sampler {
             if (lo == hi) {  // equal ones: so many, by index
                 const u64 size = MASS ? weight.mass(v_lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
                 u64 total_, at_;
-                const int i = locate([&](float v, int j) -> u64 { return v == v_lo && cut.keeps(v, first + j); },
+                const int i = locate(true, [&](float v, int j) { return v == v_lo && cut.keeps(v, first + j); }, [](float) -> u64 { return 1; },
                                      [&](u64) { return need - 1; }, total_, at_);
                 return {v_lo, i};
             }
@@ -395,30 +463,40 @@ struct Sampler {
         }
     }
 
-    // A top-k of at most S_FEW, finished in the first CTA. The k-th largest of the maxima of this CTA's
-    // threads (`largest`) bounds the k-th entry from below, so what is not below the best of the CTAs'
-    // bounds is gathered, and the rest is work on a short list. False, in all CTAs, where the list
-    // would be too long; true with the token in `id` (first CTA, one thread; else -1).
-    __device__ bool few(float largest, int k, float top_p, double min_w, float u, int &id, float &prob) {
+    // A value that the k-th largest entry of the row is not below, for k up to S_THREADS a CTA: with the
+    // largest of every thread (`largest`) at hand, each CTA takes the bucket of its ceil(k / ranks)-th
+    // largest of them, and the furthest of these buckets holds, with those before it, k entries at least.
+    __device__ float bound_of(float largest, int k) {
         for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = 0;
         if (tid == 0) sh.n_list = 0, sh.keep = S_BUCKETS - 1;
         __syncthreads();
         if (largest > -INFINITY) atomicAdd(&sh.count[bucket(largest)], 1u);
         __syncthreads();
-        const unsigned a = sh.count[2 * tid], b = sh.count[2 * tid + 1];
-        const int to = (int)scan({a + b, 0}).count;
-        if (to - (int)(a + b) < k && to >= k) sh.keep = 2 * tid + (to - (int)b < k);
+        const int a = sh.count[2 * tid], b = sh.count[2 * tid + 1], share = (k + ranks - 1) / ranks;
+        const int to = (int)scan({(u64)(a + b), 0}).count;
+        if (to - (a + b) < share && to >= share) sh.keep = 2 * tid + (to - b < share);
         __syncthreads();
         if (tid == 0) sh.part[S_WARPS].count = sh.keep;
         const int at = gather_sums();
-        int bound = S_BUCKETS - 1;
-        for (int r = 0; r < ranks; r++) bound = min(bound, (int)sh.all[at][r].count);
+        int bound = 0;
+        for (int r = 0; r < ranks; r++) bound = max(bound, (int)sh.all[at][r].count);
+        float lo, hi;
+        bucket_range(bound, lo, hi);
+        return lo;
+    }
+
+    // A top-k of at most S_FEW, finished in the first CTA: what is not below `bound` (bound_of) is
+    // gathered, and the rest is work on a short list. False, in all CTAs, where the list would be too
+    // long; true with the token in `id` (first CTA, one thread; else -1).
+    __device__ bool few(float bound, int k, float top_p, double min_w, float u, int &id, float &prob) {
         SampleShared *lead = cl.map_shared_rank(&sh, 0);
-        each([&](float v, int i) {
-            if (v > -INFINITY && bucket(v) <= bound) {
-                const unsigned at = atomicAdd(&lead->n_list, 1u);
-                if (at < S_LIST) lead->list[at] = order_of(v, first + i);
-            }
+        each([&](const float(&v)[V], int i) {
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (v[j] >= bound) {
+                    const unsigned at = atomicAdd(&lead->n_list, 1u);
+                    if (at < S_LIST) lead->list[at] = order_of(v[j], first + i + j);
+                }
         });
         cl.sync();
         const int m = (int)lead->n_list;
@@ -461,7 +539,7 @@ struct Sampler {
 };
 
 template <class T>
-__global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args p, int per) {
+__global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_args p, int per) {
     asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory");  // (the CTAs of the row have begun)
     pdl_wait();
     using S = Sampler<T>;
@@ -525,27 +603,30 @@ __global__ void __launch_bounds__(S_THREADS) sample_kernel(const sdy_sample_args
     double min_w = p.min_p ? (double)p.min_p[row] : 0.0;
     min_w = min_w != min_w ? 0.0 : min(min_w, 1.0);
     int id;
-    if (k > 0 && k <= S_FEW && k < p.n_vocab) {
+    Cut cut = {-FLT_MAX, INT_MAX};  // every finite entry and +inf
+    if (k > 0 && k < p.n_vocab) {
+        const float bound = k <= S_THREADS * ranks ? s.bound_of(largest, k) : -FLT_MAX;
         float prob;
-        if (s.few(largest, k, top_p, min_w, u, id, prob)) {
+        if (k <= S_FEW && s.few(bound, k, top_p, min_w, u, id, prob)) {
             if (id >= 0) {
                 p.id[row] = id;
                 if (p.prob) p.prob[row] = prob;
             }
             return;
         }
+        cut = s.template find_cut<false>(cut, bound, [&](Sum all) { return min((u64)k, all.count); });
     }
-    Cut cut = {-FLT_MAX, INT_MAX};  // every finite entry and +inf
-    if (k > 0 && k < p.n_vocab) cut = s.template find_cut<false>(cut, [&](Sum all) { return min((u64)k, all.count); });
     if (top_p < 1.0f)
-        cut = s.template find_cut<true>(cut, [&](Sum all) { return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1); });
+        cut = s.template find_cut<true>(cut, -FLT_MAX, [&](Sum all) {
+            return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1);
+        });
     // what is too far for min_p (or for any mass) needs no exponential
     float low = near ? (float)((double)top - (min_w > 0.0 ? fmin(S_FAR, -log(min_w)) : S_FAR) * 1.001 * (double)temp) : -FLT_MAX;
     low = fmaxf(low - 1e-5f * fabsf(low), cut.value);
     u64 total, mass;
     id = s.locate(
-        [&](float v, int i) -> u64 {
-            if (!(v >= low) || !cut.keeps(v, first + i)) return 0;
+        cut.value > -FLT_MAX || min_w > 0.0, [&](float v, int i) { return v >= low && cut.keeps(v, first + i); },
+        [&](float v) -> u64 {
             const double w = weight.scaled(v);
             return w >= min_w * MASS_ONE ? Weight::whole(w) : 0;
         },
