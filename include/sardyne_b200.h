@@ -134,7 +134,8 @@ void sdy_clear_error(void);
 /* Number of GPU kernels this process has launched through the library (for launch counting). */
 uint64_t sdy_kernel_launches(void);
 /* Nonzero when a kernel's bounded wait ran out: a tensor-core completion barrier (the kernel then
- * skipped its output and freed its tensor memory) or a fused gather's wait for the other ranks
+ * skipped its output and freed its tensor memory; sdy_tree_attention_dev's, whose output is then
+ * incomplete) or a fused gather's wait for the other ranks
  * (sdy_qmatvec_batch_f32_gather_dev). Stays set until sdy_kernel_clear_status; synchronises the
  * device. */
 uint32_t sdy_kernel_status(void);
@@ -316,8 +317,9 @@ int sdy_rope_dev(const sdy_rope_args *a, void *stream);
  *
  * n_node 1..256 (1: plain decoding), n_head a multiple of n_kv_head, head_dim a multiple of 8 up to
  * 256, every pointer 16-byte aligned, strides multiples of 16 bytes. `ws`: sdy_tree_attention_bytes
- * (which reads the counts and max_seq alone) bytes of device memory that no other call uses while
- * this one runs; nothing needs clearing. */
+ * bytes (by type, counts and head_dim; neither pointers, strides nor lengths matter) of device memory
+ * that no other call uses while this one runs: calls that may overlap, captured ones too, need one
+ * each. Nothing of it needs clearing, and nothing is kept in it from call to call. */
 typedef struct {
     int32_t type, n_seq, n_node, n_head, n_kv_head, head_dim, max_seq;
     float scale;

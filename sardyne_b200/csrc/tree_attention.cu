@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                     for (int j = 0; j < 4; j++)
                         s[i][j] += q[i].x * k[j].x + q[i].y * k[j].y + q[i].z * k[j].z + q[i].w * k[j].w;
             }
+            float f[RPT];
 #pragma unroll
             for (int i = 0; i < RPT; i++) {
                 float top = -INFINITY;
@@ -202,19 +203,23 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 #pragma unroll
                 for (int b = 8; b; b >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, b));
                 const float now = fmaxf(m[i], top), off = now == -INFINITY ? 0.0f : now;
-                const float f = exp2f(m[i] - off);  // (0 at first)
+                f[i] = exp2f(m[i] - off);  // (0 at first)
                 m[i] = now;
-                l[i] *= f;
+                float w[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float w = exp2f(s[i][j] - off);
-                    l[i] += w;
-                    P[(y * RPT + i) * (FK + 4) + x + 16 * j] = w;
+                    w[j] = exp2f(s[i][j] - off);
+                    P[(y * RPT + i) * (FK + 4) + x + 16 * j] = w[j];
                 }
-#pragma unroll
-                for (int j = 0; j < NC; j++) o[i][j].x *= f, o[i][j].y *= f, o[i][j].z *= f, o[i][j].w *= f;
+                l[i] = l[i] * f[i] + ((w[0] + w[1]) + (w[2] + w[3]));
             }
             __syncwarp();
+            // (a tile's sum on its own, then to the others': a long cache's sums err by its tiles, not its keys)
+            float4 sum[RPT][NC];
+#pragma unroll
+            for (int i = 0; i < RPT; i++)
+#pragma unroll
+                for (int j = 0; j < NC; j++) sum[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             auto products = [&](auto skip_zero) {
 #pragma unroll 2
                 for (int k = 0; k < FK; k += 4) {
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                             for (int i = 0; i < RPT; i++) {
                                 const float a = b == 0 ? w[i].x : b == 1 ? w[i].y : b == 2 ? w[i].z : w[i].w;
                                 if (skip_zero() && a == 0.0f) continue;
-                                o[i][j].x += a * v.x, o[i][j].y += a * v.y, o[i][j].z += a * v.z, o[i][j].w += a * v.w;
+                                sum[i][j].x += a * v.x, sum[i][j].y += a * v.y, sum[i][j].z += a * v.z, sum[i][j].w += a * v.w;
                             }
                         }
                     }
@@ -240,6 +245,13 @@ __global__ void __launch_bounds__(F_THREADS, 1)
             };
             if (odd) products(std::true_type());
             else products(std::false_type());
+#pragma unroll
+            for (int i = 0; i < RPT; i++)
+#pragma unroll
+                for (int j = 0; j < NC; j++) {
+                    o[i][j].x = o[i][j].x * f[i] + sum[i][j].x, o[i][j].y = o[i][j].y * f[i] + sum[i][j].y;
+                    o[i][j].z = o[i][j].z * f[i] + sum[i][j].z, o[i][j].w = o[i][j].w * f[i] + sum[i][j].w;
+                }
             __syncthreads();  // the tile has been read
         }
         const bool whole = g.t0 == 0 && g.t1 == g.tiles;
@@ -409,8 +421,9 @@ const char *counts_bad(const sdy_tree_attention_args *a) {
     return nullptr;
 }
 
+// The workspace of the shape, whichever kernel its strides choose (the tensor cores' groups are larger).
 size_t tree_bytes(const sdy_tree_attention_args &a) {
-    return tree_space(a, tree_tc_takes(a) ? tree_tc_rows(a) : fp32_rows(a)).bytes;
+    return tree_space(a, a.type != T_F32 && a.head_dim <= TC_MAX_DIM ? tree_tc_rows(a) : fp32_rows(a)).bytes;
 }
 
 bool tree_check(const sdy_tree_attention_args *a) {

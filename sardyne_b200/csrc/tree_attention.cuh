@@ -8,6 +8,7 @@ namespace sdy {
 
 constexpr int TA_MAX_NODES = 256;
 constexpr int TA_MAX_DIM = 256;
+constexpr int TC_MAX_DIM = 128;  // of the tensor-core kernel
 
 // The split. A row group is the rows (node, query head) of one KV head of one sequence that a CTA
 // holds at once. Its work is its tiles of keys and, unless every tile finds a CTA of its own,

@@ -386,7 +386,8 @@ __global__ void __launch_bounds__(TT, 1)
         const int st = (warp - 4) / 4, tid = threadIdx.x - 128 - 128 * st;  // stream, row of its tile
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;                  // 32 lanes to a warp
         const uint32_t tm_s = tmem + TM_S + st * 128 + lanes, tm_o = tmem + TM_O + st * 128 + lanes;
-        const float c = fabsf(p.scale) * 1.4426950408889634f;
+        // (a scale of zero: queries of zero, since a masked score's -inf times zero would be NaN)
+        const float c = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
         const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
         const int chunks = p.head_dim / 8;  // 16-byte pieces of a row
         int base = 0, arrived = 0, seg = 0;  // loads, arrivals and segments before this one
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(TT, 1)
                 for (int i = 0; i < PER; i++) {
                     const int r = i * (32 / PER) + lane / PER;
                     const int64_t at = __shfl_sync(~0u, q_at, r);
-                    v[i] = r < rows_left && j < chunks ? __ldg((const uint4 *)((const T *)p.q + at) + j) : make_uint4(0, 0, 0, 0);
+                    v[i] = r < rows_left && j < chunks && p.scale != 0.0f ? __ldg((const uint4 *)((const T *)p.q + at) + j) : make_uint4(0, 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
@@ -722,7 +723,7 @@ void tc_pick(const sdy_tree_attention_args &a, const TreeSpace &sp, const CUtens
 
 bool tree_tc_takes(const sdy_tree_attention_args &a) {
     auto mappable = [](int64_t stride, int64_t count) { return count == 1 || (stride > 0 && stride < (int64_t)1 << 39); };
-    return a.type != T_F32 && a.head_dim <= 128 && mappable(a.cache_row, a.max_seq) && mappable(a.cache_head, a.n_kv_head) &&
+    return a.type != T_F32 && a.head_dim <= TC_MAX_DIM && mappable(a.cache_row, a.max_seq) && mappable(a.cache_head, a.n_kv_head) &&
            mappable(a.cache_seq, a.n_seq);
 }
 

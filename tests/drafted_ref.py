@@ -95,7 +95,9 @@ def sample(row, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         return int(order[0]), 1.0
     top = row[order[0]]
     with np.errstate(invalid="ignore", over="ignore"):
-        w = np.where(row[order] == top, 1.0, np.exp((row[order] - top) / temperature))
+        # (an infinite logit takes all the weight, whatever the temperature)
+        far = -np.inf if np.isinf(top) else 0.0
+        w = np.where(row[order] == top, 1.0, np.exp(far if far else (row[order] - top) / temperature))
     n = len(order)
     if top_k > 0:
         n = min(n, top_k)

@@ -122,6 +122,9 @@ def test_tree_attention_refusals(change, word):
 
 def test_tree_attention_bytes():
     lib = capi.lib()
+    for shape in (dict(), dict(head_dim=256, q_head=256, out_head=256), dict(type=0), dict(n_head=40, n_node=200)):
+        need = lib.sdy_tree_attention_bytes(ctypes.byref(tree_args(**shape)))
+        assert need == lib.sdy_tree_attention_bytes(ctypes.byref(tree_args(**{**shape, "cache_seq": 0, "q": 0, "ws": 0, "max_seq": 7})))
     assert lib.sdy_tree_attention_bytes(ctypes.byref(tree_args(max_seq=1 << 20))) > 0
     assert lib.sdy_tree_attention_bytes(ctypes.byref(tree_args(n_node=300))) == 0 and "n_node" in capi.last_error()
     lib.sdy_clear_error()

@@ -374,6 +374,42 @@ def test_tree_attention_large_scores(kind):
         check_tree(kind, q, (f64(k), f64(v)), n_past, None, 1.0, out)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-12])
+def test_tree_attention_scales(kind, scale):
+    """A scale of zero (all keys alike, masked ones none the less out), below zero, and tiny."""
+    q, k, v, n_past, parent, par, clean = tree_case(kind, 2, 11, 4, 2, 64, [150, 5], seed=8)
+    out = torch.full_like(q, float("nan"))
+    call(capi.lib().sdy_tree_attention_dev, tree_args(kind, q, k, v, n_past, parent, out, scale))
+    check_tree(kind, q, clean, n_past, par, float(np.float32(scale)), out)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_tree_attention_shared_cache(kind):
+    """A sequence stride of zero: all sequences read one cache (it holds the same drafted rows too)."""
+    g = gen(16)
+    q = randn(g, 3, 5, 4, 64, kind=kind)
+    k, v = (randn(g, 1, 2, 140, 64, kind=kind).expand(3, 2, 140, 64) for _ in range(2))
+    n_past = torch.tensor([130, 7, 64], dtype=torch.int32, device="cuda")
+    out = torch.full_like(q, float("nan"))
+    call(capi.lib().sdy_tree_attention_dev, tree_args(kind, q, k, v, n_past, None, out, 0.125))
+    check_tree(kind, q, (f64(k), f64(v)), n_past, None, 0.125, out)
+
+
+def test_tree_attention_many_sequences():
+    """More sequences than threads of a block, most of them short: every share holds several."""
+    n_seq = 900
+    past = [(37 * s) % 300 for s in range(n_seq)]
+    for kind in ("bf16", "f32"):
+        g = gen(17)
+        q = randn(g, n_seq, 2, 2, 64, kind=kind)
+        k, v = randn(g, n_seq, 1, 302, 64, kind=kind), randn(g, n_seq, 1, 302, 64, kind=kind)
+        n_past = torch.tensor(past, dtype=torch.int32, device="cuda")
+        out = torch.full_like(q, float("nan"))
+        call(capi.lib().sdy_tree_attention_dev, tree_args(kind, q, k, v, n_past, None, out, 0.125))
+        check_tree(kind, q, (f64(k), f64(v)), n_past, None, 0.125, out)
+
+
 def test_tree_attention_far_offsets():
     """Elements past 2^32 of a cache in HBM: the last sequence's rows lie behind them."""
     n_seq, kv, dim = 3, 1, 64
@@ -459,6 +495,39 @@ def test_sample_ties(kind):
     for s in (dict(), dict(top_k=40), dict(top_k=9000), dict(top_p=0.5), dict(top_p=0.25, top_k=64), dict(min_p=1.0),
               dict(min_p=0.2), dict(top_p=0.0), dict(temperature=0.0), dict(temperature=1e-30), dict(temperature=1e30)):
         check_sample(x, u, sample(x, u, kind, **s), **s)
+
+
+@pytest.mark.parametrize("spread", [1e-2, 1e-5, 30.0])
+def test_sample_narrow_and_wide(spread):
+    """Logits so close that a bucket of distances holds thousands of different ones, and far apart."""
+    g = gen(21)
+    rows, vocab = 6, 50001
+    x = randn(g, rows, vocab) * spread
+    u = torch.rand(rows, generator=g, device="cuda").cpu().numpy()
+    for s in (dict(), dict(top_k=7), dict(top_k=511), dict(top_k=512), dict(top_k=513), dict(top_k=20000), dict(top_p=0.3),
+              dict(top_p=0.999), dict(top_k=30000, top_p=0.5, min_p=0.01), dict(temperature=0.01, top_p=0.9)):
+        check_sample(x, u, sample(x, u, **s), **s)
+
+
+def test_sample_zeros_of_both_signs():
+    """-0 and 0 are the same logit: the lower index goes first."""
+    x = torch.full((4, 64), -1.0, device="cuda")
+    x[:, 9], x[:, 30], x[:, 31] = -0.0, 0.0, -0.0
+    u = np.array([0.0, 0.3, 0.6, 0.9], np.float32)
+    for s in (dict(top_k=1), dict(top_k=2), dict(top_k=3), dict(temperature=0.0), dict(top_p=0.1), dict(min_p=1.0)):
+        got = sample(x, u, **s)
+        check_sample(x + 0.0, u, got, **s)
+    assert (sample(x, u, temperature=0.0)[0] == 9).all()
+
+
+def test_sample_infinite_temperature():
+    """All weights alike; an infinite logit still takes everything."""
+    x = torch.linspace(-5, 5, 1000, device="cuda").repeat(3, 1)
+    x[1, 17] = float("inf")
+    x[2, ::2] = -float("inf")
+    u = np.array([0.25, 0.5, 0.75], np.float32)
+    for s in (dict(), dict(top_k=10), dict(top_p=0.5), dict(min_p=0.5)):
+        check_sample(x, u, sample(x, u, temperature=float("inf"), **s), temperature=float("inf"), **s)
 
 
 def test_sample_special_values():
