@@ -55,7 +55,8 @@ template <class T, int RPT, int NC>
 __global__ void __launch_bounds__(F_THREADS, 1)
     tree_fp32_kernel(const sdy_tree_attention_args p, const Fp32Layout lay, Cut *cuts, float *part_o, float2 *part_ml) {
     constexpr int R = 16 * RPT;
-    __shared__ int64_t scan[F_THREADS / 32], found[8];
+    __shared__ int64_t scan[F_THREADS / 32 + 8];
+    int64_t found[8];
     __shared__ int16_t up[TA_MAX_NODES];
     __shared__ uint32_t path[TA_MAX_NODES][TA_MAX_NODES / 32 + 1];  // the nodes each node sees; 0: padding
     extern __shared__ __align__(16) float mem[];
@@ -97,10 +98,14 @@ __global__ void __launch_bounds__(F_THREADS, 1)
         if (lay.stages == 2) fetch(g.t0, 0);
         for (int w = tid; w < R * quads; w += F_THREADS) {
             const int r = w / quads, e = 4 * (w - r * quads), row = g.group * R + r, node = row / rep;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (row < rows) v = load4((const T *)p.q + g.s * p.q_seq + node * p.q_node + (g.head * rep + row - node * rep) * p.q_head + e);
-            *(float4 *)(Q + r * ld + e) = v;
+            const T *q = (const T *)p.q + g.s * p.q_seq + node * p.q_node + (g.head * rep + row - node * rep) * p.q_head + e;
+            float *to = Q + r * ld + e;
+            if (row >= rows) *(float4 *)to = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            else if (std::is_same<T, float>::value)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(q) : "memory");
+            else *(float4 *)to = load4(q);
         }
+        if (lay.stages == 2) asm volatile("cp.async.commit_group;\n" ::: "memory");
         if (edges) {
             if (tid < 32) load_tree(up, parent, p.n_node);
             __syncthreads();
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
             const int st = lay.stages == 2 ? (t - g.t0) & 1 : 0, j0 = t * FK;
             if (lay.stages == 2) {
                 if (t + 1 < g.t1) {
-                    fetch(t + 1, st ^ 1);
+                    fetch(t + 1, st ^ 1);  // (its group is the last: what came before, the queries too, is waited for)
                     asm volatile("cp.async.wait_group 1;\n" ::: "memory");
                 } else {
                     asm volatile("cp.async.wait_group 0;\n" ::: "memory");

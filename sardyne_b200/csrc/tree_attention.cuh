@@ -103,7 +103,7 @@ struct Share {
     const sdy_tree_attention_args &p;
     int64_t u, end, base;   // next unit, end, units of the sequences before s
     int s, tiles, past, items, setup;  // items: row groups per sequence; setup: units before a group's tiles
-    __device__ Share(const sdy_tree_attention_args &p_, const int64_t *found, int items_)
+    __device__ Share(const sdy_tree_attention_args &p_, const int64_t (&found)[8], int items_)
         : p(p_), u(found[0]), end(found[1]), base(found[3]), s((int)found[2]), tiles((int)found[4]),
           past((int)found[6]), items(items_), setup((int)found[7]) {}
     // The next run; runs that hold no tile (only the end of a row group's setup) are passed over.
@@ -134,25 +134,45 @@ struct Share {
     }
 };
 
-// Where CTA `cta`'s share begins, found by the whole block (THREADS threads, all of them): the
-// units before each run of sequences by a scan over the threads, the rest by walking that run.
-// out[0..7] = first unit, end, first sequence, units before it, its tiles, all units, its length, the
-// setup.
+// Where CTA `cta`'s share begins, for all threads of the block: out[0..7] = first unit, end, first
+// sequence, units before it, its tiles, all units, its length, the setup. Up to 32 sequences are
+// found by every warp for itself; more by a scan over the block's threads, each with a run of sequences.
 template <int KEYS, int THREADS>
 __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int items, int cta,
-                                           int64_t *scan /* THREADS / 32 */, int64_t *out) {
-    const int t = threadIdx.x, run = (p.n_seq + THREADS - 1) / THREADS;
+                                           int64_t *scan /* shared, THREADS / 32 + 8 */, int64_t (&out)[8]) {
+    const int t = threadIdx.x, lane = t % 32;
+    auto tiles_at = [&](int past) { return (lengths_of(p, 0, past).keys + KEYS - 1) / KEYS; };
+    auto past_of = [&](int s) { return max(p.n_past[s], 0); };
+    if (p.n_seq <= 32) {
+        const int past = lane < p.n_seq ? past_of(lane) : 0, mine = lane < p.n_seq ? tiles_at(past) : 0;
+        int sum = mine;  // inclusive (fewer than 2^25 tiles to a sequence)
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const int total = __shfl_sync(~0u, sum, 31), setup = (int64_t)total * items <= TA_CTAS ? 0 : TA_SETUP;
+        const int64_t units = ((int64_t)total + p.n_seq * setup) * items;
+        const int64_t u0 = share_begin(units, cta), u1 = share_begin(units, cta + 1);
+        const int before = sum - mine + lane * setup;
+        const unsigned here = __ballot_sync(~0u, lane < p.n_seq && (int64_t)before * items <= u0);
+        const int s = 31 - __clz(here);  // the last sequence that begins by u0
+        out[0] = u0, out[1] = u1, out[2] = s, out[3] = (int64_t)__shfl_sync(~0u, before, s) * items;
+        out[4] = __shfl_sync(~0u, mine, s), out[5] = units, out[6] = __shfl_sync(~0u, past, s), out[7] = setup;
+        return;
+    }
+    const int run = (p.n_seq + THREADS - 1) / THREADS;
     const int s0 = min(t * run, p.n_seq), s1 = min(s0 + run, p.n_seq);
-    auto tiles_of = [&](int s) { return (lengths_of(p, s).keys + KEYS - 1) / KEYS; };
     int64_t mine = 0;
-    for (int s = s0; s < s1; s++) mine += tiles_of(s);
-    int64_t sum = mine;  // inclusive over the warp
+    for (int s = s0; s < s1; s++) mine += tiles_at(past_of(s));
+    int64_t sum = mine, *said = scan + THREADS / 32;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int64_t v = __shfl_up_sync(~0u, sum, o);
-        if (t % 32 >= o) sum += v;
+        if (lane >= o) sum += v;
     }
-    if (t % 32 == 31) scan[t / 32] = sum;
-    if (t == 0) out[2] = out[3] = out[4] = out[6] = 0;
+    if (lane == 31) scan[t / 32] = sum;
+    if (t < 8) said[t] = 0;
     __syncthreads();
     int64_t before = 0, total = 0;
 #pragma unroll
@@ -165,23 +185,26 @@ __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int
     mine += (int64_t)(s1 - s0) * setup;
     const int64_t units = (total + (int64_t)p.n_seq * setup) * items;
     const int64_t u0 = share_begin(units, cta), u1 = share_begin(units, cta + 1);
-    if (t == 0) out[0] = u0, out[1] = u1, out[5] = units, out[7] = setup;
     if (u0 < u1 && u0 >= before * items && u0 < (before + mine) * items) {
-        int s = s0, n = run == 1 ? (int)mine - setup : tiles_of(s0);
+        int s = s0, past = past_of(s0), n = tiles_at(past);
         int64_t b = before * items;
         while (u0 >= b + (int64_t)(n + setup) * items) {
             b += (int64_t)(n + setup) * items;
             s++;
-            n = tiles_of(s);
+            past = past_of(s);
+            n = tiles_at(past);
         }
-        out[2] = s, out[3] = b, out[4] = n, out[6] = max(p.n_past[s], 0);
+        said[2] = s, said[3] = b, said[4] = n, said[6] = past;
     }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; i++) out[i] = said[i];
+    out[0] = u0, out[1] = u1, out[5] = units, out[7] = setup;
 }
 // What CTA `cta` notes for join_kernel (one thread, after find_share).
 template <int KEYS>
-__device__ __forceinline__ void note_cut(const sdy_tree_attention_args &p, int items, int groups, int cta, const int64_t *found,
-                                         Cut *cuts) {
+__device__ __forceinline__ void note_cut(const sdy_tree_attention_args &p, int items, int groups, int cta,
+                                         const int64_t (&found)[8], Cut *cuts) {
     Cut cut = {0, 0, 0, 0};
     Share<KEYS> share(p, found, items);
     Segment g;

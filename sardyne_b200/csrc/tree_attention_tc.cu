@@ -51,7 +51,7 @@ struct Shared {
     uint64_t merge_full, merge_done, drain;
     uint32_t tmem;
     int odd;  // the last segment (from 1) whose drafted V rows hold NaN or infinities
-    int64_t scan[TT / 32], share[8];
+    int64_t scan[TT / 32 + 8];
     int16_t up[2][TA_MAX_NODES];  // per stream (its warps are in one segment while they walk)
     float2 ml[TR];
 };
@@ -250,13 +250,15 @@ __global__ void __launch_bounds__(TT, 1)
         sh.odd = 0;
     }
     pdl_wait();
-    find_share<TK, TT>(p, p.n_kv_head * groups, blockIdx.x, sh.scan, sh.share);
+    int64_t found[8];
+    find_share<TK, TT>(p, p.n_kv_head * groups, blockIdx.x, sh.scan, found);
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = sh.tmem;
-    Share<TK> share(p, sh.share, p.n_kv_head * groups);
+    Share<TK> share(p, found, p.n_kv_head * groups);
     Segment g;
+    bool more = share.next(g, groups);  // (the first run here, by the same instructions in all roles)
 
     // registers go to the two warpgroups that hold rows: 72 x 128 + 216 x 256 <= 168 x 384
     if (warp < 4) {
@@ -275,7 +277,7 @@ __global__ void __launch_bounds__(TT, 1)
                 pos[r]++;
                 return true;
             };
-            while (ok && share.next(g, groups)) {
+            for (; ok && more; more = share.next(g, groups)) {
                 const int n = g.t1 - g.t0;
 #pragma unroll
                 for (int r = 0; r < STEP; r++)
@@ -287,9 +289,9 @@ __global__ void __launch_bounds__(TT, 1)
 #pragma unroll
                     for (int r = 0; r < STEP; r++) {  // V, and the K that follows it, arrive together
                         if (i * STEP + r >= n) continue;
-                        const bool more = (i + 1) * STEP + r < n;
-                        ok = ok && load(&vmap, r, i, more ? 2 * TILE : TILE);
-                        if (more) ok = ok && load(&kmap, r, i + 1, 0);
+                        const bool last = (i + 1) * STEP + r >= n;
+                        ok = ok && load(&vmap, r, i, last ? TILE : 2 * TILE);
+                        if (!last) ok = ok && load(&kmap, r, i + 1, 0);
                         event[r]++;
                     }
                 }
@@ -300,9 +302,9 @@ __global__ void __launch_bounds__(TT, 1)
                     for (int q = max(0, event[r] - NS); q < event[r]; q++) mbar_wait(&sh.full[r * NS + q % NS], q / NS & 1);
             }
         }
-        if (warp == 3 && lane == 0) note_cut<TK>(p, p.n_kv_head * groups, groups, blockIdx.x, sh.share, cuts);
+        if (warp == 3 && lane == 0) note_cut<TK>(p, p.n_kv_head * groups, groups, blockIdx.x, found, cuts);
         if (warp == 3) {  // the queries of the share into L2, ahead of the loads that keep HBM busy
-            while (share.next(g, groups)) {
+            for (; more; more = share.next(g, groups)) {
                 const int first = g.group * ROWS, last = min(rows, first + ROWS);
                 for (int r = first + lane; r < last; r += 32) {
                     const int node = r / rep;
@@ -337,7 +339,7 @@ __global__ void __launch_bounds__(TT, 1)
                     if (!DUAL || st == 1) mma_commit(free);
                 }
             };
-            while (ok && share.next(g, groups)) {
+            for (; ok && more; more = share.next(g, groups)) {
                 const int all = g.t1 - g.t0;
                 auto tiles = [&](int st) { return DUAL ? all : (all + 1 - st) / 2; };  // of a stream
                 for (int st = 0; ok && st < NQ; st++) ok = warp_wait(&sh.q_ready[st], seg & 1);
@@ -353,11 +355,11 @@ __global__ void __launch_bounds__(TT, 1)
 #pragma unroll
                     for (int st = 0; st < 2; st++) {
                         if (!ok || i >= tiles(st)) continue;
-                        const bool more = i + 1 < tiles(st);
+                        const bool last = i + 1 == tiles(st);
                         const int v_slot = slot_of(st, pos[st]), k_slot = slot_of(st, pos[st] + 1);
                         const uint32_t v = uniform(v_lo + v_slot * (TILE >> 4)), k = uniform(k_lo + k_slot * (TILE >> 4)), again = uniform(i > 0);
                         if (!DUAL || st == 0) ok = wait_full(st, event[st]);
-                        pos[st] += more ? 2 : 1, event[st]++;
+                        pos[st] += last ? 1 : 2, event[st]++;
                         ok = ok && warp_wait(&sh.p_ready[st], p_parity >> st & 1);
                         if (!ok) continue;
                         p_parity ^= 1u << st;
@@ -367,9 +369,9 @@ __global__ void __launch_bounds__(TT, 1)
 #pragma unroll
                             for (int c = 0; c < TK / 16; c++) mma_ts(d, a + 8 * c, v + (2048 * c >> 4), id_pv, c > 0 ? 1u : again);
                             if (!DUAL || st == 1) mma_commit(&sh.empty[v_slot]);
-                            if (!more) mma_commit(&sh.o_done[st]);
+                            if (last) mma_commit(&sh.o_done[st]);
                         }
-                        if (more) qk(st, k, &sh.empty[k_slot]);  // over P, which the MMAs before have read by then
+                        if (!last) qk(st, k, &sh.empty[k_slot]);  // over P, which the MMAs before have read by then
                     }
                 }
                 seg++;
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(TT, 1)
         int base = 0, arrived = 0, seg = 0;  // loads, arrivals and segments before this one
         uint32_t s_parity = 0, o_parity = 0;
         bool ok = true;
-        while (ok && share.next(g, groups)) {
+        for (; ok && more; more = share.next(g, groups)) {
             const int n = (g.t1 - g.t0 + STEP - 1 - (DUAL ? 0 : st)) / STEP;  // the stream's tiles
             const Lengths len = lengths_of(p, g.s, g.past);
             const int32_t *parent = p.parent ? p.parent + (int64_t)g.s * p.n_node : nullptr;
@@ -411,18 +413,25 @@ __global__ void __launch_bounds__(TT, 1)
                 constexpr int PER = HC * 8;  // lanes to a row: 16 bytes each
                 uint8_t *dst = qbuf + (DUAL ? st : 0) * QTILE + (warp % 4) * 32 * 128;
                 const int j = lane % PER, rows_left = rows - (row - lane);
-                uint4 v[PER];
+                // (copies, so that all are in flight at once; what is no query is zero)
 #pragma unroll
                 for (int i = 0; i < PER; i++) {
                     const int r = i * (32 / PER) + lane / PER;
                     const int64_t at = __shfl_sync(~0u, q_at, r);
-                    v[i] = r < rows_left && j < chunks && p.scale != 0.0f ? __ldg((const uint4 *)((const T *)p.q + at) + j) : make_uint4(0, 0, 0, 0);
+                    const bool some = r < rows_left && j < chunks && p.scale != 0.0f;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(
+                                     smem_u32(dst + r * 128 + (j / 8) * QCHUNK + (((j & 7) ^ (r & 7)) << 4))),
+                                 "l"((const uint4 *)((const T *)p.q + (some ? at : 0)) + (some ? j : 0)), "r"(some ? 16 : 0)
+                                 : "memory");
                 }
-#pragma unroll
-                for (int i = 0; i < PER; i++) {
-                    const int r = i * (32 / PER) + lane / PER;
-                    v[i].x ^= flip, v[i].y ^= flip, v[i].z ^= flip, v[i].w ^= flip;
-                    *(uint4 *)(dst + r * 128 + (j / 8) * QCHUNK + (((j & 7) ^ (r & 7)) << 4)) = v[i];
+                asm volatile("cp.async.wait_all;\n" ::: "memory");
+                if (flip) {
+#pragma unroll 1
+                    for (int i = 0; i < PER; i++) {
+                        const int r = i * (32 / PER) + lane / PER;
+                        uint4 *x = (uint4 *)(dst + r * 128 + (j / 8) * QCHUNK + (((j & 7) ^ (r & 7)) << 4));
+                        *x = make_uint4(x->x ^ flip, x->y ^ flip, x->z ^ flip, x->w ^ flip);
+                    }
                 }
                 fence_async_smem();
                 mbar_arrive(&sh.q_ready[st]);
