@@ -134,6 +134,12 @@ struct Sampler {
             at(v, i * V);
         }
     }
+    // f(value) for the entries of `mask`, a lane's own of the V from index i on, by whole warps: few of them
+    // one after the other, each lane at its next (f's second argument: whether it has one).
+    template <class F> __device__ __forceinline__ void few_of(unsigned mask, int most, int i, F f) const {
+        for (int k = 0; k < most; k++, mask &= mask - 1)
+            f(mask ? to_f32(((const T *)sample_row)[i + __ffs(mask) - 1]) : weight.top, mask != 0);
+    }
     // The values that can be in bucket b (and a few around): what is outside need not be placed.
     __device__ __forceinline__ void bucket_range(int b, float &lo, float &hi) const {
         const float slack = 1e-6f * (fabsf(weight.top) + (b + 1) / scale);
@@ -239,27 +245,28 @@ struct Sampler {
     // The index at which the running sum of of(value) over the entries in(value, index here), in index
     // order, passes want_of(total); the sum of all and the one there in `total` and `at`.
     template <class In, class Of, class W>
-    __device__ int locate(bool sparse, In in, Of of, W want_of, u64 &total, u64 &at) {
+    __device__ int locate(In in, Of of, W want_of, u64 &total, u64 &at) {
         // a warp's entries are a run of indexes, in steps of 32 reads, whose sums it notes
         u64 *steps = sh.sorted + warp * 32;
         const int per = (n / V + S_WARPS - 1) / S_WARPS, i0 = min(warp * per, n / V), i1 = min(i0 + per, n / V);
         auto vec = [&](int i) -> u64 {  // by whole warps
             float v[V];
-            bool ok[V], any = false;
+            unsigned mask = 0;
             read(i, i1, v);
 #pragma unroll
-            for (int j = 0; j < V; j++) ok[j] = in(v[j], i * V + j), any = any || ok[j];
+            for (int j = 0; j < V; j++) mask |= in(v[j], i * V + j) ? 1u << j : 0u;
+            const int most = __reduce_max_sync(~0u, __popc(mask));
             u64 sum = 0;
-            if (!__any_sync(~0u, any)) return sum;
-            if (sparse) {  // (few are in: entry by entry)
-#pragma unroll
-                for (int j = 0; j < V; j++)
-                    if (ok[j]) sum += of(v[j]);
+            if (2 * most <= V) {
+                few_of(mask, most, i * V, [&](float x, bool has) {
+                    const u64 m = of(x);
+                    sum += has ? m : 0;
+                });
             } else {
 #pragma unroll
                 for (int j = 0; j < V; j++) {
                     const u64 m = of(v[j]);
-                    sum += ok[j] ? m : 0;
+                    sum += mask >> j & 1 ? m : 0;
                 }
             }
             return sum;
@@ -323,7 +330,6 @@ struct Sampler {
     template <bool MASS, class Target>
     __device__ Cut find_cut(Cut cut, float bound, Target target_of) {
         float v_hi = weight.top, v_lo = fmaxf(cut.value, bound);  // the values in question
-        const bool sparse = cut.value > -FLT_MAX;
         unsigned k_hi = 0;                         // key of v_hi, and buckets by key >> shift from it
         int shift = -1;                            // (at first, buckets by distance)
         Sum done = {0, 0};                         // before them
@@ -336,29 +342,31 @@ struct Sampler {
             __syncthreads();
             unsigned far = 0;  // by distance, the last bucket has most entries (and none of them mass)
             each([&](const float(&v)[V], int i) {
-                bool ok[V], any = false;
+                unsigned mask = 0;
 #pragma unroll
-                for (int j = 0; j < V; j++) ok[j] = in_question(v[j], i + j), any = any || ok[j];
-                if (!__any_sync(~0u, any)) return;
+                for (int j = 0; j < V; j++) mask |= in_question(v[j], i + j) ? 1u << j : 0u;
+                const int most = __reduce_max_sync(~0u, __popc(mask));
+                auto count = [&](bool has, int b, u64 m) {
+                    const bool last = shift < 0 && b == S_BUCKETS - 1;
+                    far += has && last;
+                    if (!has || last) return;
+                    atomicAdd(&sh.count[b], 1u);
+                    if (MASS) {
+                        const unsigned low = (unsigned)m, old = atomicAdd(&sh.lo[b], low);
+                        const unsigned high = (unsigned)(m >> 32) + (old + low < low);
+                        if (high) atomicAdd(&sh.hi[b], high);
+                    }
+                };
+                if (2 * most <= V) {
+                    few_of(mask, most, i, [&](float x, bool has) { count(has, place(x), MASS ? weight.mass(x) : 0); });
+                    return;
+                }
                 int b[V];
                 u64 m[V];
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    b[j] = place(v[j]);
-                    m[j] = MASS && (!sparse || ok[j]) ? weight.mass(v[j]) : 0;
-                }
+                for (int j = 0; j < V; j++) b[j] = place(v[j]), m[j] = MASS ? weight.mass(v[j]) : 0;
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const bool last = shift < 0 && b[j] == S_BUCKETS - 1;
-                    far += ok[j] && last;
-                    if (!ok[j] || last) continue;
-                    atomicAdd(&sh.count[b[j]], 1u);
-                    if (MASS) {
-                        const unsigned low = (unsigned)m[j], old = atomicAdd(&sh.lo[b[j]], low);
-                        const unsigned high = (unsigned)(m[j] >> 32) + (old + low < low);
-                        if (high) atomicAdd(&sh.hi[b[j]], high);
-                    }
-                }
+                for (int j = 0; j < V; j++) count(mask >> j & 1, b[j], m[j]);
             });
             for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(~0u, far, o);
             if (lane == 0 && far) atomicAdd(&sh.count[S_BUCKETS - 1], far);
@@ -454,7 +462,7 @@ struct Sampler {
             if (lo == hi) {  // equal ones: so many, by index
                 const u64 size = MASS ? weight.mass(v_lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
                 u64 total_, at_;
-                const int i = locate(true, [&](float v, int j) { return v == v_lo && cut.keeps(v, first + j); }, [](float) -> u64 { return 1; },
+                const int i = locate([&](float v, int j) { return v == v_lo && cut.keeps(v, first + j); }, [](float) -> u64 { return 1; },
                                      [&](u64) { return need - 1; }, total_, at_);
                 return {v_lo, i};
             }
@@ -625,7 +633,7 @@ __global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_a
     low = fmaxf(low - 1e-5f * fabsf(low), cut.value);
     u64 total, mass;
     id = s.locate(
-        cut.value > -FLT_MAX || min_w > 0.0, [&](float v, int i) { return v >= low && cut.keeps(v, first + i); },
+        [&](float v, int i) { return v >= low && cut.keeps(v, first + i); },
         [&](float v) -> u64 {
             const double w = weight.scaled(v);
             return w >= min_w * MASS_ONE ? Weight::whole(w) : 0;

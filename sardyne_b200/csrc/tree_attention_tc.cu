@@ -1,23 +1,31 @@
 // Tree attention over 16-bit caches on the tensor cores (tcgen05, accumulators in TMEM).
 //
 // For one KV head of one sequence the rows are its (node, query head) pairs, 128 to an MMA tile;
-// per tile of 80 keys, S = Q K^T (128 x 80, f32 in TMEM), P = 2^(c S - m) as 16-bit values in TMEM,
-// O += P V with P as the A operand. m is a row's running maximum; O and the sum are rescaled only
-// when it has grown by more than 2^8 since it was last set (the division by the sum takes out any
-// common factor; 2^8 keeps P inside the range of f16), which after the first tiles hardly ever
-// happens, so O stays in TMEM.
+// per tile of 128 keys, S = Q K^T (128 x 128, f32 in TMEM), P = 2^(c S - m) as 16-bit values over S's
+// own columns, O += P V with P as the A operand. P takes the type of V because one tcgen05.mma has one
+// type for both; its rounding (2^-9 of a probability in bf16, 2^-12 in f16) is of the size of the
+// output's own and adds to it as independent errors do: 1.4 times the output's rounding in all. m is a
+// row's running maximum; O and the sum are rescaled only when it has grown by more than 2^8 since it
+// was last set (the division by the sum takes out any common factor; 2^8 keeps P inside the range of
+// f16), which after the first tiles hardly ever happens, so O stays in TMEM.
 //
-// One CTA per SM, twelve warps: a TMA producer (K and V tiles through a ring of shared memory
-// slots), an MMA issuer, and two streams of four warps that turn S into P, one row to a thread. With
-// more than 128 rows the streams hold two row tiles and share every K and V tile (DUAL); with fewer
-// they share the rows and take the tiles in turn, and the first stream joins the two results at the
-// end. 80 keys: S and P then fit side by side beside O in a stream's half of TMEM (80 + 40 of 128
-// columns), so the next S is formed while the exponentials of this one run; with tiles of 128 keys and
-// P over S's own columns each stream waited for P V and the next Q K^T in turn, 3400 cycles per 2 x 128
-// rows and 128 keys (measured on B200, 2 x 64 nodes, 32 heads, 65537 keys).
+// One CTA per SM, twelve warps: a TMA producer (K and V tiles through rings of shared memory slots),
+// an MMA issuer, one that notes the cuts and fetches queries ahead, and two streams of four warps that
+// turn S into P, one row to a thread. With more than 128 rows the streams hold two row tiles and share
+// every K and V tile (DUAL); with fewer they share the rows and take the tiles in turn, and the first
+// stream joins the two results at the end.
 //
-// Bound by the exponentials (16 a cycle) and the shared memory reads of Q K^T alike from about 256
-// rows, by HBM below about 64.
+// What bounds it, for many rows, is a stream's cycle: the exponentials (128 x 128 at 16 a cycle are 1024
+// cycles; with the reads of S, the maxima and the stores of P 2000), then P V and the next Q K^T (512
+// cycles each alone; Q K^T reads 128 bytes of shared memory a cycle, all there is, and loses some to the
+// arriving tiles), the other stream's MMAs under this one's exponentials: 3360 cycles per 2 x 128 rows
+// and 128 keys, 0.61 of the tensor pipe's rate, and the power limit then holds the clock near 1.66 GHz (2
+// sequences of 64 nodes and 32 heads over 65537 keys: 165 us, 830 TFLOP/s). Tried and slower: S of 80
+// keys beside P, with the next Q K^T under the exponentials (four waits more per key, and a wait on a
+// barrier that is complete takes 100 to 200 cycles of an issuer that cannot run ahead: 4100 cycles per
+// 128 keys); the scores in four parts, each part's maximum under the one before's exponentials (a
+// vote per part: 3900). For few rows it is bound by latency: about 12 us from the launch to the last store,
+// of which loading the queries, the first tile and storing the result take 2 us each.
 #include "tree_attention.cuh"
 
 #include <cuda.h>
@@ -35,7 +43,8 @@ constexpr int TR = 128;       // rows per MMA tile
 constexpr int TT = 384;       // threads
 constexpr int CHUNK = TK * 128, QCHUNK = TR * 128;  // bytes of 64 elements of a tile's rows, 128-byte swizzled
 constexpr int WAIT_LIMIT = 1 << 22;  // mbarrier polls before giving up (about a second)
-constexpr uint32_t TM_S = 0, TM_O = 256;     // TMEM columns of stream 0's S (and P over it) and O; stream 1's are 128 on
+// TMEM columns of stream 0's S (and P over it) and O; stream 1's are 128 on.
+constexpr uint32_t TM_S = 0, TM_O = 256;
 constexpr float GROWTH = 8.0f;
 
 __device__ unsigned g_tree_status;  // nonzero: a wait ran out
@@ -316,7 +325,7 @@ __global__ void __launch_bounds__(TT, 1)
         if (warp == 1) {
             // One warp issues for both streams in turn, which keeps them out of step: the one's MMAs run
             // under the other's exponentials (with a warp for each they fall into step and share both
-            // pipes: 4600 cycles per unit instead of 3600). The whole warp waits, one lane issues; the
+            // pipes: 4600 cycles per 128 keys instead of 3400). The whole warp waits, one lane issues; the
             // shuffles tell the compiler that the operands are the same in all lanes (the tensor
             // instructions take them from uniform registers).
             auto uniform = [](uint32_t x) { return __shfl_sync(~0u, x, 0); };
