@@ -134,6 +134,21 @@ struct Sampler {
             at(v, i * V);
         }
     }
+    // Which of V entries lie in [lo, hi], one bit each.
+    __device__ __forceinline__ static unsigned within(const float (&v)[V], float lo, float hi) {
+        unsigned mask = 0;
+#pragma unroll
+        for (int j = 0; j < V; j++) mask |= v[j] >= lo && v[j] <= hi ? 1u << j : 0u;
+        return mask;
+    }
+    // Of `mask`, the entries from index i here on, what `cut` keeps (it holds none below the cut's value).
+    __device__ __forceinline__ unsigned kept(const Cut &cut, const float (&v)[V], int i, unsigned mask) const {
+        if (cut.index < INT_MAX)
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (v[j] == cut.value && first + i + j > cut.index) mask &= ~(1u << j);
+        return mask;
+    }
     // f(value) for the entries of `mask`, a lane's own of the V from index i on, by whole warps: few of them
     // one after the other, each lane at its next (f's second argument: whether it has one).
     template <class F> __device__ __forceinline__ void few_of(unsigned mask, int most, int i, F f) const {
@@ -242,19 +257,17 @@ struct Sampler {
         __syncthreads();
     }
 
-    // The index at which the running sum of of(value) over the entries in(value, index here), in index
-    // order, passes want_of(total); the sum of all and the one there in `total` and `at`.
-    template <class In, class Of, class W>
-    __device__ int locate(In in, Of of, W want_of, u64 &total, u64 &at) {
+    // The index at which the running sum of of(value) over the entries in [lo, hi] that `cut` keeps, in
+    // index order, passes want_of(total); the sum of all and the one there in `total` and `at`.
+    template <class Of, class W>
+    __device__ int locate(float lo, float hi, const Cut &cut, Of of, W want_of, u64 &total, u64 &at) {
         // a warp's entries are a run of indexes, in steps of 32 reads, whose sums it notes
         u64 *steps = sh.sorted + warp * 32;
         const int per = (n / V + S_WARPS - 1) / S_WARPS, i0 = min(warp * per, n / V), i1 = min(i0 + per, n / V);
         auto vec = [&](int i) -> u64 {  // by whole warps
             float v[V];
-            unsigned mask = 0;
             read(i, i1, v);
-#pragma unroll
-            for (int j = 0; j < V; j++) mask |= in(v[j], i * V + j) ? 1u << j : 0u;
+            const unsigned mask = kept(cut, v, i * V, within(v, lo, hi));
             const int most = __reduce_max_sync(~0u, __popc(mask));
             u64 sum = 0;
             if (2 * most <= V) {
@@ -308,7 +321,7 @@ struct Sampler {
                 c += to_here - m;
                 for (int j = i * V;; j++) {
                     const float x = to_f32(((const T *)sample_row)[j]);
-                    const u64 one = in(x, j) ? of(x) : 0;
+                    const u64 one = x >= lo && x <= hi && cut.keeps(x, first + j) ? of(x) : 0;
                     if (want < c + one) {
                         v[0] = first + j, v[1] = one;
                         break;
@@ -335,16 +348,13 @@ struct Sampler {
         Sum done = {0, 0};                         // before them
         u64 target = 0;
         while (true) {
-            auto in_question = [&](float v, int i) { return v >= v_lo && v <= v_hi && cut.keeps(v, first + i); };
             auto place = [&](float v) { return shift < 0 ? bucket(v) : (int)((k_hi - key_of(v)) >> shift); };
             for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
             unsigned far = 0;  // by distance, the last bucket has most entries (and none of them mass)
             each([&](const float(&v)[V], int i) {
-                unsigned mask = 0;
-#pragma unroll
-                for (int j = 0; j < V; j++) mask |= in_question(v[j], i + j) ? 1u << j : 0u;
+                const unsigned mask = kept(cut, v, i, within(v, v_lo, v_hi));
                 const int most = __reduce_max_sync(~0u, __popc(mask));
                 auto count = [&](bool has, int b, u64 m) {
                     const bool last = shift < 0 && b == S_BUCKETS - 1;
@@ -407,15 +417,19 @@ struct Sampler {
             done = {got[1], got[2]};
             float lo_v = v_lo, hi_v = v_hi;
             if (shift < 0) bucket_range(crossing, lo_v, hi_v);
-            lo_v = fmaxf(lo_v, v_lo);
-            auto is_crossing = [&](float v, int i) { return v >= lo_v && v <= hi_v && in_question(v, i) && place(v) == crossing; };
+            lo_v = fmaxf(lo_v, v_lo), hi_v = fminf(hi_v, v_hi);
+            auto crossing_ones = [&](auto f) {
+                each([&](const float(&v)[V], int i) {
+                    for (unsigned mask = kept(cut, v, i, within(v, lo_v, hi_v)); mask; mask &= mask - 1) {
+                        const int j = i + __ffs(mask) - 1;
+                        const float x = to_f32(((const T *)sample_row)[j]);
+                        if (place(x) == crossing) f(x, j);
+                    }
+                });
+            };
             if (got[3] <= S_LIST) {  // gathered and ranked in the first CTA
                 SampleShared *lead = cl.map_shared_rank(&sh, 0);
-                each([&](const float(&v)[V], int i) {
-#pragma unroll
-                    for (int j = 0; j < V; j++)
-                        if (is_crossing(v[j], i + j)) lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(v[j], first + i + j);
-                });
+                crossing_ones([&](float x, int i) { lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(x, first + i); });
                 cl.sync();
                 bool found = false;
                 u64 w[4] = {0, 0, 0, 0};
@@ -439,11 +453,7 @@ struct Sampler {
             }
             // too many for the list: the range of their keys into buckets again
             unsigned lo = ~0u, hi = 0;
-            each([&](const float(&v)[V], int i) {
-#pragma unroll
-                for (int j = 0; j < V; j++)
-                    if (is_crossing(v[j], i + j)) lo = min(lo, key_of(v[j])), hi = max(hi, key_of(v[j]));
-            });
+            crossing_ones([&](float x, int) { lo = min(lo, key_of(x)), hi = max(hi, key_of(x)); });
             for (int o = 16; o; o >>= 1) {
                 lo = min(lo, __shfl_xor_sync(~0u, lo, o));
                 hi = max(hi, __shfl_xor_sync(~0u, hi, o));
@@ -462,8 +472,7 @@ struct Sampler {
             if (lo == hi) {  // equal ones: so many, by index
                 const u64 size = MASS ? weight.mass(v_lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
                 u64 total_, at_;
-                const int i = locate([&](float v, int j) { return v == v_lo && cut.keeps(v, first + j); }, [](float) -> u64 { return 1; },
-                                     [&](u64) { return need - 1; }, total_, at_);
+                const int i = locate(v_lo, v_lo, cut, [](float) -> u64 { return 1; }, [&](u64) { return need - 1; }, total_, at_);
                 return {v_lo, i};
             }
             k_hi = hi;
@@ -499,12 +508,11 @@ struct Sampler {
     __device__ bool few(float bound, int k, float top_p, double min_w, float u, int &id, float &prob) {
         SampleShared *lead = cl.map_shared_rank(&sh, 0);
         each([&](const float(&v)[V], int i) {
-#pragma unroll
-            for (int j = 0; j < V; j++)
-                if (v[j] >= bound) {
-                    const unsigned at = atomicAdd(&lead->n_list, 1u);
-                    if (at < S_LIST) lead->list[at] = order_of(v[j], first + i + j);
-                }
+            for (unsigned mask = within(v, bound, INFINITY); mask; mask &= mask - 1) {
+                const int j = i + __ffs(mask) - 1;
+                const unsigned at = atomicAdd(&lead->n_list, 1u);
+                if (at < S_LIST) lead->list[at] = order_of(to_f32(((const T *)sample_row)[j]), first + j);
+            }
         });
         cl.sync();
         const int m = (int)lead->n_list;
@@ -633,7 +641,7 @@ __global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_a
     low = fmaxf(low - 1e-5f * fabsf(low), cut.value);
     u64 total, mass;
     id = s.locate(
-        [&](float v, int i) { return v >= low && cut.keeps(v, first + i); },
+        low, INFINITY, cut,
         [&](float v) -> u64 {
             const double w = weight.scaled(v);
             return w >= min_w * MASS_ONE ? Weight::whole(w) : 0;
