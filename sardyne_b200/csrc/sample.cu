@@ -38,7 +38,8 @@ constexpr int S_MAX_VOCAB = SAMPLE_MAX_VOCAB;
 constexpr int S_CLUSTER = 8;                   // CTAs to a row, at most
 constexpr int S_BUCKETS = 1024, S_LIST = 1024;  // the list: entries ranked at once
 constexpr int S_FEW = 512;                     // a top-k that the first CTA finishes alone, one entry to a thread
-constexpr double S_SCALE = 32.0;               // buckets per unit of (max - l) / T
+constexpr double S_SCALE = 32.0;               // buckets per unit of (max - l) / T, for numbers of entries
+constexpr int S_STEPS = 16;                    // steps of ln 2 / 256 to a bucket, for masses
 constexpr double S_FAR = 31.3;                 // exp(-31.3) 2^44 < 1/2: no mass from here on
 constexpr double MASS_ONE = 17592186044416.0;  // 2^44
 typedef unsigned long long u64;
@@ -54,20 +55,14 @@ __device__ __forceinline__ u64 order_of(float x, int i) { return (u64)key_of(x) 
 __device__ __forceinline__ float value_of(u64 order) { return value_of((unsigned)(order >> 32)); }
 __device__ __forceinline__ int index_of(u64 order) { return (int)~(unsigned)order; }
 
-struct Sum {
-    u64 count, mass;
-    __device__ Sum operator+(const Sum &o) const { return {count + o.count, mass + o.mass}; }
-};
-__device__ __forceinline__ Sum shfl_up(Sum v, int o) { return {__shfl_up_sync(~0u, v.count, o), __shfl_up_sync(~0u, v.mass, o)}; }
-
 struct SampleShared {
-    unsigned count[S_BUCKETS], lo[S_BUCKETS], hi[S_BUCKETS];  // of this CTA's entries (mass in two words)
-    u64 list[S_LIST], sorted[S_LIST];                         // first CTA: gathered entries
+    unsigned lo[S_BUCKETS], hi[S_BUCKETS];  // this CTA's entries: their number, or mass in two words
+    u64 list[S_LIST], sorted[S_LIST];       // first CTA: gathered entries
     unsigned n_list, keep;
-    Sum part[S_WARPS + 1];                                    // per warp, then the CTA
-    Sum all[2][S_CLUSTER];                                    // exchanged, by rank; two in turn
-    u64 said[2][4];                                           // what one CTA tells the others; two in turn
-    double power[256];                                        // 2^(j/256)
+    u64 part[S_WARPS + 1];                  // sums per warp, then the CTA's
+    u64 all[2][S_CLUSTER];                  // exchanged, by rank; two in turn
+    u64 said[2][2];                         // what one CTA tells the others; two in turn
+    double power[256];                      // 2^(44 + j/256)
 };
 __shared__ SampleShared sh;  // (by name, so that accesses are known to be to shared memory)
 extern __shared__ __align__(16) uint8_t sample_row[];
@@ -76,21 +71,27 @@ extern __shared__ __align__(16) uint8_t sample_row[];
 // whole and |f| <= 1/2, and w = 2^(k/256) 2^(f/256), the second factor by its series to f^4 (the rest is
 // below 2^-53).
 struct Weight {
-    float top;          // the largest logit
-    double m, inv, by;  // the same; 1 / temperature; 256 / (temperature ln 2)
-    // 2^44 w, and 0 for what rounds to no whole number
-    __device__ __forceinline__ double scaled(float v) const {
-        constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
-        constexpr double C = 0.0027076061740622863;   // ln 2 / 256
-        const double d = (double)v - m;
-        const double t = fma(d, by, MAGIC), kd = t - MAGIC, f = fma(d, by, -kd);
+    float top, far;  // the largest logit; no mass up to `far` (below top)
+    double m, by;    // the largest (at most FLT_MAX); 256 / (temperature ln 2)
+    static constexpr double MAGIC = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the nearest integer
+    __device__ __forceinline__ double distance(float v) const { return (double)fminf(v, FLT_MAX) - m; }
+    __device__ __forceinline__ int steps(float v) const { return -__double2loint(fma(distance(v), by, MAGIC)); }
+    // 2^44 w, and 0 for what rounds to no whole number; -k in `steps`
+    __device__ __forceinline__ double scaled(float v, int &steps) const {
+        constexpr double C = 0.0027076061740622863;  // ln 2 / 256
+        const double d = distance(v), t = fma(d, by, MAGIC), f = fma(d, by, MAGIC - t);
         const int k = __double2loint(t);
         double e = fma(f, C * C * C * C / 24, C * C * C / 6);
         e = fma(e, f, C * C / 2);
         e = fma(e, f, C);
         e = fma(e, f, 1.0) * sh.power[k & 255];
-        e = __longlong_as_double(__double_as_longlong(e) + ((long long)((k >> 8) + 44) << 52));
-        return v == top ? MASS_ONE : d * inv > -S_FAR ? e : 0.0;  // (no branch: a thread's entries go abreast)
+        steps = -k;
+        e = __hiloint2double(__double2hiint(e) + ((k & ~255) << 12), __double2loint(e));
+        return v > far ? e : 0.0;  // (no branch: a thread's entries go abreast)
+    }
+    __device__ __forceinline__ double scaled(float v) const {
+        int steps;
+        return scaled(v, steps);
     }
     __device__ __forceinline__ static u64 whole(double m) {  // nearest integer, below 2^51
         return (u64)__double_as_longlong(m + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
@@ -156,39 +157,46 @@ struct Sampler {
             f(mask ? to_f32(((const T *)sample_row)[i + __ffs(mask) - 1]) : weight.top, mask != 0);
     }
     // The values that can be in bucket b (and a few around): what is outside need not be placed.
-    __device__ __forceinline__ void bucket_range(int b, float &lo, float &hi) const {
+    template <bool MASS> __device__ __forceinline__ void bucket_range(int b, float &lo, float &hi) const {
+        if (MASS) {
+            lo = __double2float_rd(weight.m - (S_STEPS * b + S_STEPS) / weight.by);
+            hi = b ? __double2float_ru(weight.m - (S_STEPS * b - 1) / weight.by) : INFINITY;
+            return;
+        }
         const float slack = 1e-6f * (fabsf(weight.top) + (b + 1) / scale);
         lo = near && b < S_BUCKETS - 1 ? weight.top - (b + 0.51f) / scale - slack : -FLT_MAX;
         hi = near ? weight.top - (b - 0.51f) / scale + slack : INFINITY;
     }
-    // Buckets by distance from the largest; the last one's entries have no mass.
-    __device__ __forceinline__ int bucket(float v) const {
-        const float x = near ? (weight.top - v) * scale : (float)fmin((weight.m - (double)v) * weight.inv * S_SCALE, 1e6);
+    // Buckets by distance from the largest: for masses by the steps of the exponential, for numbers in 32
+    // bits where the range allows it, the last one from 32 units on.
+    template <bool MASS> __device__ __forceinline__ int bucket(float v) const {
+        if (MASS) return (int)((unsigned)weight.steps(v) / S_STEPS);
+        const float x = near ? (weight.top - v) * scale : (float)fmin(-weight.distance(v) * weight.by * (S_SCALE * 0.0027076061740622863), 1e6);
         const int b = (int)(__float_as_uint(fminf(x, S_BUCKETS - 1.0f) + 8388608.0f) & (S_BUCKETS - 1));
         return v == weight.top ? 0 : b;
     }
 
     // v summed over the threads of the CTA up to and with this one; the CTA's sum in sh.part[S_WARPS].
-    __device__ Sum scan(Sum v) {
-        Sum in = v;
+    __device__ u64 scan(u64 v) {
+        u64 in = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const Sum u = shfl_up(in, o);
+            const u64 u = __shfl_up_sync(~0u, in, o);
             if (lane >= o) in = in + u;
         }
         __syncthreads();
         if (lane == 31) sh.part[warp] = in;
         __syncthreads();
-        Sum below = {0, 0}, total = {0, 0};
+        u64 below = 0, total = 0;
 #pragma unroll
         for (int w = 0; w < S_WARPS; w++) {
-            if (w < warp) below = below + sh.part[w];
-            total = total + sh.part[w];
+            if (w < warp) below += sh.part[w];
+            total += sh.part[w];
         }
         if (tid == 0) sh.part[S_WARPS] = total;
         return below + in;
     }
-    // One Sum of every CTA, sh.part[S_WARPS], to all: in sh.all[the result].
+    // One number of every CTA, sh.part[S_WARPS], to all: in sh.all[the result].
     __device__ int gather_sums() {
         __syncthreads();
         if (tid < ranks) cl.map_shared_rank(&sh, tid)->all[turn][rank] = sh.part[S_WARPS];
@@ -197,30 +205,50 @@ struct Sampler {
         return turn ^ 1;
     }
     // The sums of the CTAs of lower rank and of all.
-    __device__ void exchange(Sum &before, Sum &total) {
+    __device__ void exchange(u64 &before, u64 &total) {
         const int at = gather_sums();
-        before = total = {0, 0};
+        before = total = 0;
         for (int r = 0; r < ranks; r++) {
-            if (r < rank) before = before + sh.all[at][r];
-            total = total + sh.all[at][r];
+            if (r < rank) before += sh.all[at][r];
+            total += sh.all[at][r];
         }
     }
-    // Four numbers from the one thread in the cluster whose `mine` is set, to all; its warp stores them.
-    __device__ void tell(bool mine, const u64 (&v)[4], u64 (&got)[4]) {
+    // Two numbers from the one thread in the cluster whose `mine` is set, to all; its warp stores them.
+    __device__ void tell(bool mine, u64 a, u64 b, u64 (&got)[2]) {
         const unsigned who = __ballot_sync(~0u, mine);
         if (who) {
-            u64 word = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const u64 x = __shfl_sync(~0u, v[i], __ffs(who) - 1);
-                if (lane % 4 == i) word = x;
-            }
-            if (lane / 4 < ranks) cl.map_shared_rank(&sh, lane / 4)->said[told][lane % 4] = word;
+            a = __shfl_sync(~0u, a, __ffs(who) - 1);
+            b = __shfl_sync(~0u, b, __ffs(who) - 1);
+            if (lane / 2 < ranks) cl.map_shared_rank(&sh, lane / 2)->said[told][lane % 2] = lane % 2 ? b : a;
         }
         cl.sync();
-#pragma unroll
-        for (int i = 0; i < 4; i++) got[i] = sh.said[told][i];
+        got[0] = sh.said[told][0], got[1] = sh.said[told][1];
         told ^= 1;
+    }
+    // The entries in [lo, hi] that `cut` keeps and in(value) holds for, added to the first CTA's list: a
+    // warp's together. Their number, in all CTAs; what is behind S_LIST is not in the list.
+    template <class In> __device__ unsigned gather(float lo, float hi, const Cut &cut, In in) {
+        SampleShared *lead = cl.map_shared_rank(&sh, 0);
+        each([&](const float(&v)[V], int i) {
+            unsigned mask = kept(cut, v, i, within(v, lo, hi));
+            if (!__any_sync(~0u, mask)) return;
+            for (unsigned m = mask; m; m &= m - 1)
+                if (!in(to_f32(((const T *)sample_row)[i + __ffs(m) - 1]))) mask ^= m & -m;
+            int at = __popc(mask);
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(~0u, at, o);
+                if (lane >= o) at += u;
+            }
+            unsigned from = lane == 31 && at ? atomicAdd(&lead->n_list, (unsigned)at) : 0;
+            from = __shfl_sync(~0u, from, 31) + at - __popc(mask);
+            for (; mask && from < S_LIST; mask &= mask - 1, from++) {
+                const int j = i + __ffs(mask) - 1;
+                lead->list[from] = order_of(to_f32(((const T *)sample_row)[j]), first + j);
+            }
+        });
+        cl.sync();
+        return lead->n_list;
     }
     // The first CTA's list of m entries in descending order: sorted bitonically, one entry to a thread,
     // or, where there are more, every one counts the ones before it.
@@ -294,13 +322,12 @@ struct Sampler {
             mine += m;
             if (lane == 0) steps[k] = m;
         }
-        const Sum to = scan({0, lane == 31 ? mine : 0});
-        Sum before, sum;
-        exchange(before, sum);
-        total = sum.mass;
-        const u64 want = want_of(total), end = before.mass + __shfl_sync(~0u, to.mass, 31), begin = end - mine;
+        const u64 to = scan(lane == 31 ? mine : 0);
+        u64 before;
+        exchange(before, total);
+        const u64 want = want_of(total), end = before + __shfl_sync(~0u, to, 31), begin = end - mine;
         bool here = false;
-        u64 v[4] = {0, 0, 0, 0};
+        u64 v[2] = {0, 0};
         if (want >= begin && want < end) {
             auto prefix = [&](u64 m) {
 #pragma unroll
@@ -331,8 +358,8 @@ struct Sampler {
             }
             __syncwarp();
         }
-        u64 got[4];
-        tell(here, v, got);
+        u64 got[2];
+        tell(here, v[0], v[1], got);
         at = got[1];
         return (int)got[0];
     }
@@ -343,134 +370,123 @@ struct Sampler {
     template <bool MASS, class Target>
     __device__ Cut find_cut(Cut cut, float bound, Target target_of) {
         float v_hi = weight.top, v_lo = fmaxf(cut.value, bound);  // the values in question
+        if (MASS) v_lo = fmaxf(v_lo, nextafterf(weight.far, INFINITY));
         unsigned k_hi = 0;                         // key of v_hi, and buckets by key >> shift from it
         int shift = -1;                            // (at first, buckets by distance)
-        Sum done = {0, 0};                         // before them
-        u64 target = 0;
+        u64 done = 0, target = 0;                  // the sum before them; the one to reach
         while (true) {
-            auto place = [&](float v) { return shift < 0 ? bucket(v) : (int)((k_hi - key_of(v)) >> shift); };
-            for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = sh.lo[b] = sh.hi[b] = 0;
+            auto place = [&](float v) { return shift < 0 ? bucket<MASS>(v) : (int)((k_hi - key_of(v)) >> shift); };
+            for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.lo[b] = sh.hi[b] = 0;
             if (tid == 0) sh.n_list = 0;
             __syncthreads();
-            unsigned far = 0;  // by distance, the last bucket has most entries (and none of them mass)
+            unsigned far = 0;  // by distance, the last bucket has most entries
             each([&](const float(&v)[V], int i) {
                 const unsigned mask = kept(cut, v, i, within(v, v_lo, v_hi));
                 const int most = __reduce_max_sync(~0u, __popc(mask));
-                auto count = [&](bool has, int b, u64 m) {
-                    const bool last = shift < 0 && b == S_BUCKETS - 1;
-                    far += has && last;
-                    if (!has || last) return;
-                    atomicAdd(&sh.count[b], 1u);
+                auto add = [&](bool has, int b, u64 m) {
                     if (MASS) {
+                        if (!has) return;
                         const unsigned low = (unsigned)m, old = atomicAdd(&sh.lo[b], low);
                         const unsigned high = (unsigned)(m >> 32) + (old + low < low);
                         if (high) atomicAdd(&sh.hi[b], high);
+                    } else {
+                        const bool last = shift < 0 && b == S_BUCKETS - 1;
+                        far += has && last;
+                        if (has && !last) atomicAdd(&sh.lo[b], 1u);
                     }
                 };
+                auto both = [&](float x, int &b) -> u64 {
+                    if (!MASS) return b = place(x), 1;
+                    int steps;
+                    const u64 m = Weight::whole(weight.scaled(x, steps));
+                    b = shift < 0 ? (int)((unsigned)steps / S_STEPS) : place(x);
+                    return m;
+                };
                 if (2 * most <= V) {
-                    few_of(mask, most, i, [&](float x, bool has) { count(has, place(x), MASS ? weight.mass(x) : 0); });
+                    few_of(mask, most, i, [&](float x, bool has) {
+                        int b;
+                        const u64 m = both(x, b);
+                        add(has, b, m);
+                    });
                     return;
                 }
                 int b[V];
                 u64 m[V];
 #pragma unroll
-                for (int j = 0; j < V; j++) b[j] = place(v[j]), m[j] = MASS ? weight.mass(v[j]) : 0;
+                for (int j = 0; j < V; j++) m[j] = both(v[j], b[j]);
 #pragma unroll
-                for (int j = 0; j < V; j++) count(mask >> j & 1, b[j], m[j]);
+                for (int j = 0; j < V; j++) add(mask >> j & 1, b[j], m[j]);
             });
-            for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(~0u, far, o);
-            if (lane == 0 && far) atomicAdd(&sh.count[S_BUCKETS - 1], far);
+            if (!MASS) {
+                for (int o = 16; o; o >>= 1) far += __shfl_xor_sync(~0u, far, o);
+                if (lane == 0 && far) atomicAdd(&sh.lo[S_BUCKETS - 1], far);
+            }
             cl.sync();
             // this CTA merges a run of buckets, two to a thread at most
             const int run = S_BUCKETS / ranks, per = (run + S_THREADS - 1) / S_THREADS, b0 = rank * run + tid * per;
-            Sum own[2] = {{0, 0}, {0, 0}};
+            u64 own[2] = {0, 0};
 #pragma unroll
             for (int j = 0; j < 2; j++)
                 if (j < per && tid * per + j < run)
                     for (int r = 0; r < ranks; r++) {
                         const SampleShared *o = cl.map_shared_rank(&sh, r);
-                        own[j].count += o->count[b0 + j];
-                        if (MASS) own[j].mass += (u64)o->hi[b0 + j] << 32 | o->lo[b0 + j];
+                        own[j] += MASS ? (u64)o->hi[b0 + j] << 32 | o->lo[b0 + j] : o->lo[b0 + j];
                     }
-            const Sum to = scan(own[0] + own[1]);
-            Sum before, total;
+            u64 c = scan(own[0] + own[1]), before, total;
             exchange(before, total);
             if (shift < 0) target = target_of(total);
             // the bucket in which the sum reaches the target
-            bool here = false;
-            u64 v[4] = {0, 0, 0, 0};
-            Sum c = done + before + to;
-            c = {c.count - own[0].count - own[1].count, c.mass - own[0].mass - own[1].mass};
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const u64 from = MASS ? c.mass : c.count;
-                const Sum next = c + own[j];
-                if (!here && from < target && target <= (MASS ? next.mass : next.count)) {
-                    here = true;
-                    v[0] = b0 + j, v[1] = c.count, v[2] = c.mass, v[3] = own[j].count;
-                }
-                c = next;
-            }
-            u64 got[4];
-            tell(here, v, got);
+            c += done + before - own[0] - own[1];
+            const bool one = c < target && target <= c + own[0], two = c + own[0] < target && target <= c + own[0] + own[1];
+            u64 got[2];
+            tell(one || two, b0 + two, two ? c + own[0] : c, got);
             const int crossing = (int)got[0];
-            done = {got[1], got[2]};
+            done = got[1];
             float lo_v = v_lo, hi_v = v_hi;
-            if (shift < 0) bucket_range(crossing, lo_v, hi_v);
+            if (shift < 0) bucket_range<MASS>(crossing, lo_v, hi_v);
             lo_v = fmaxf(lo_v, v_lo), hi_v = fminf(hi_v, v_hi);
-            auto crossing_ones = [&](auto f) {
-                each([&](const float(&v)[V], int i) {
-                    for (unsigned mask = kept(cut, v, i, within(v, lo_v, hi_v)); mask; mask &= mask - 1) {
-                        const int j = i + __ffs(mask) - 1;
-                        const float x = to_f32(((const T *)sample_row)[j]);
-                        if (place(x) == crossing) f(x, j);
-                    }
-                });
-            };
-            if (got[3] <= S_LIST) {  // gathered and ranked in the first CTA
-                SampleShared *lead = cl.map_shared_rank(&sh, 0);
-                crossing_ones([&](float x, int i) { lead->list[atomicAdd(&lead->n_list, 1u)] = order_of(x, first + i); });
-                cl.sync();
+            auto crosses = [&](float x) { return place(x) == crossing; };
+            const unsigned m = gather(lo_v, hi_v, cut, crosses);
+            if (m <= S_LIST) {  // ranked in the first CTA
                 bool found = false;
-                u64 w[4] = {0, 0, 0, 0};
+                u64 w = 0;
                 if (rank == 0) {
-                    const int m = (int)got[3];
-                    rank_list(m);
-                    Sum e[2];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const int i = 2 * tid + j;
-                        e[j] = i < m ? Sum{1, MASS ? weight.mass(value_of(sh.sorted[i])) : 0} : Sum{0, 0};
-                    }
-                    const Sum upto = done + scan(e[0] + e[1]);
-                    const u64 second = MASS ? upto.mass : upto.count, one = second - (MASS ? e[1].mass : e[1].count);
-                    const u64 none = one - (MASS ? e[0].mass : e[0].count);
-                    if (none < target && target <= one) found = true, w[0] = sh.sorted[2 * tid];
-                    else if (one < target && target <= second) found = true, w[0] = sh.sorted[2 * tid + 1];
+                    rank_list((int)m);
+                    const unsigned i = 2 * tid;
+                    const u64 e0 = i < m ? MASS ? weight.mass(value_of(sh.sorted[i])) : 1 : 0;
+                    const u64 e1 = i + 1 < m ? MASS ? weight.mass(value_of(sh.sorted[i + 1])) : 1 : 0;
+                    const u64 second = done + scan(e0 + e1), first_ = second - e1, none = first_ - e0;
+                    found = none < target && target <= second;
+                    if (found) w = sh.sorted[i + (first_ < target)];
                 }
-                tell(found, w, got);
+                tell(found, w, 0, got);
                 return {value_of(got[0]), index_of(got[0])};
             }
             // too many for the list: the range of their keys into buckets again
             unsigned lo = ~0u, hi = 0;
-            crossing_ones([&](float x, int) { lo = min(lo, key_of(x)), hi = max(hi, key_of(x)); });
+            each([&](const float(&v)[V], int i) {
+                for (unsigned mask = kept(cut, v, i, within(v, lo_v, hi_v)); mask; mask &= mask - 1) {
+                    const float x = to_f32(((const T *)sample_row)[i + __ffs(mask) - 1]);
+                    if (crosses(x)) lo = min(lo, key_of(x)), hi = max(hi, key_of(x));
+                }
+            });
             for (int o = 16; o; o >>= 1) {
                 lo = min(lo, __shfl_xor_sync(~0u, lo, o));
                 hi = max(hi, __shfl_xor_sync(~0u, hi, o));
             }
             __syncthreads();
-            if (lane == 0) sh.part[warp] = {lo, hi};
+            if (lane == 0) sh.part[warp] = (u64)lo << 32 | hi;
             __syncthreads();
             if (tid == 0) {
-                for (int j = 1; j < S_WARPS; j++) lo = min(lo, (unsigned)sh.part[j].count), hi = max(hi, (unsigned)sh.part[j].mass);
-                sh.part[S_WARPS] = {lo, hi};
+                for (int j = 1; j < S_WARPS; j++) lo = min(lo, (unsigned)(sh.part[j] >> 32)), hi = max(hi, (unsigned)sh.part[j]);
+                sh.part[S_WARPS] = (u64)lo << 32 | hi;
             }
             const int at = gather_sums();
             lo = ~0u, hi = 0;
-            for (int r = 0; r < ranks; r++) lo = min(lo, (unsigned)sh.all[at][r].count), hi = max(hi, (unsigned)sh.all[at][r].mass);
+            for (int r = 0; r < ranks; r++) lo = min(lo, (unsigned)(sh.all[at][r] >> 32)), hi = max(hi, (unsigned)sh.all[at][r]);
             v_lo = value_of(lo), v_hi = value_of(hi);
             if (lo == hi) {  // equal ones: so many, by index
-                const u64 size = MASS ? weight.mass(v_lo) : 1, need = (target - (MASS ? done.mass : done.count) + size - 1) / size;
+                const u64 size = MASS ? weight.mass(v_lo) : 1, need = (target - done + size - 1) / size;
                 u64 total_, at_;
                 const int i = locate(v_lo, v_lo, cut, [](float) -> u64 { return 1; }, [&](u64) { return need - 1; }, total_, at_);
                 return {v_lo, i};
@@ -484,21 +500,21 @@ struct Sampler {
     // largest of every thread (`largest`) at hand, each CTA takes the bucket of its ceil(k / ranks)-th
     // largest of them, and the furthest of these buckets holds, with those before it, k entries at least.
     __device__ float bound_of(float largest, int k) {
-        for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.count[b] = 0;
+        for (int b = tid; b < S_BUCKETS; b += S_THREADS) sh.lo[b] = 0;
         if (tid == 0) sh.n_list = 0, sh.keep = S_BUCKETS - 1;
         __syncthreads();
-        if (largest > -INFINITY) atomicAdd(&sh.count[bucket(largest)], 1u);
+        if (largest > -INFINITY) atomicAdd(&sh.lo[bucket<false>(largest)], 1u);
         __syncthreads();
-        const int a = sh.count[2 * tid], b = sh.count[2 * tid + 1], share = (k + ranks - 1) / ranks;
-        const int to = (int)scan({(u64)(a + b), 0}).count;
+        const int a = sh.lo[2 * tid], b = sh.lo[2 * tid + 1], share = (k + ranks - 1) / ranks;
+        const int to = (int)scan(a + b);
         if (to - (a + b) < share && to >= share) sh.keep = 2 * tid + (to - b < share);
         __syncthreads();
-        if (tid == 0) sh.part[S_WARPS].count = sh.keep;
+        if (tid == 0) sh.part[S_WARPS] = sh.keep;
         const int at = gather_sums();
         int bound = 0;
-        for (int r = 0; r < ranks; r++) bound = max(bound, (int)sh.all[at][r].count);
+        for (int r = 0; r < ranks; r++) bound = max(bound, (int)sh.all[at][r]);
         float lo, hi;
-        bucket_range(bound, lo, hi);
+        bucket_range<false>(bound, lo, hi);
         return lo;
     }
 
@@ -506,16 +522,7 @@ struct Sampler {
     // gathered, and the rest is work on a short list. False, in all CTAs, where the list would be too
     // long; true with the token in `id` (first CTA, one thread; else -1).
     __device__ bool few(float bound, int k, float top_p, double min_w, float u, int &id, float &prob) {
-        SampleShared *lead = cl.map_shared_rank(&sh, 0);
-        each([&](const float(&v)[V], int i) {
-            for (unsigned mask = within(v, bound, INFINITY); mask; mask &= mask - 1) {
-                const int j = i + __ffs(mask) - 1;
-                const unsigned at = atomicAdd(&lead->n_list, 1u);
-                if (at < S_LIST) lead->list[at] = order_of(to_f32(((const T *)sample_row)[j]), first + j);
-            }
-        });
-        cl.sync();
-        const int m = (int)lead->n_list;
+        const int m = (int)min(gather(bound, INFINITY, {-FLT_MAX, INT_MAX}, [](float) { return true; }), S_LIST + 1u);
         cl.sync();  // (read by all: the first CTA may write it again, or leave)
         if (m > S_LIST) return false;
         id = -1;
@@ -526,9 +533,9 @@ struct Sampler {
         const double w = tid < kept_k ? weight.scaled(value_of(sh.sorted[tid])) : 0.0;
         const u64 mass = Weight::whole(w);
         if (tid == 0) sh.keep = kept_k;
-        const u64 upto = scan({0, mass}).mass;
+        const u64 upto = scan(mass);
         __syncthreads();
-        const u64 all = sh.part[S_WARPS].mass;
+        const u64 all = sh.part[S_WARPS];
         if (top_p < 1.0f) {
             const u64 target = max((u64)ceil(max((double)top_p, 0.0) * (double)all), (u64)1);
             if (upto - mass < target && target <= upto) atomicMin(&sh.keep, (unsigned)tid + 1);
@@ -536,11 +543,11 @@ struct Sampler {
         if (tid > 0 && tid < kept_k && w < min_w * MASS_ONE) atomicMin(&sh.keep, (unsigned)tid);
         __syncthreads();
         const int keep = (int)sh.keep;
-        if (tid == keep - 1) sh.part[S_WARPS].mass = upto;
+        if (tid == keep - 1) sh.part[S_WARPS] = upto;
         u64 *masses = sh.list;
         if (tid < keep) masses[tid] = mass;
         __syncthreads();
-        const u64 total = sh.part[S_WARPS].mass;
+        const u64 total = sh.part[S_WARPS];
         const double at_u = (u > 0.0f ? (double)u : 0.0) * (double)total;
         const u64 want = at_u >= (double)total ? total - 1 : (u64)at_u;
         if (tid < keep) {
@@ -565,7 +572,7 @@ __global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_a
     constexpr int V = S::V;
     const int first = min(rank * per, p.n_vocab), n = min(per, p.n_vocab - first), full = (n + V - 1) / V * V;
     const T *x = (const T *)p.logits + row * p.row_stride + first;
-    if (tid < 256) sh.power[tid] = exp2(tid / 256.0);
+    if (tid < 256) sh.power[tid] = exp2(44 + tid / 256.0);
 
     // The row into shared memory (NaN as -inf, -0 as 0), and its largest entry: each thread meets its
     // own in rising order, so the first of equal ones stays.
@@ -588,16 +595,16 @@ __global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_a
     for (int i = vec * V + tid; i < full; i += S_THREADS) ((T *)sample_row)[i] = take(i < n ? x[i] : from_f32<T>(-INFINITY), i);
     u64 best = order_of(largest, first + where);
     for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
-    if (lane == 0) sh.part[warp].mass = best;
+    if (lane == 0) sh.part[warp] = best;
     __syncthreads();
     asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory");
     if (tid < ranks) {
-        for (int j = 0; j < S_WARPS; j++) best = max(best, sh.part[j].mass);
-        cl.map_shared_rank(&sh, tid)->all[1][rank].mass = best;
+        for (int j = 0; j < S_WARPS; j++) best = max(best, sh.part[j]);
+        cl.map_shared_rank(&sh, tid)->all[1][rank] = best;
     }
     cl.sync();
     best = 0;
-    for (int r = 0; r < ranks; r++) best = max(best, sh.all[1][r].mass);
+    for (int r = 0; r < ranks; r++) best = max(best, sh.all[1][r]);
 
     const float top = value_of(best);
     const float temp = p.temperature ? p.temperature[row] : 1.0f;
@@ -609,11 +616,11 @@ __global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_a
         return;  // (nobody reads this CTA's shared memory any more)
     }
     // (an infinite largest logit: the others are infinitely far whatever the temperature)
-    const double inv = isinf(top) ? 1.0 : 1.0 / (double)temp;
-    const Weight weight{top, (double)top, inv, inv * 369.32993046757463};  // 256 / ln 2
+    const double t = isinf(top) ? 1.0 : (double)temp, m = (double)fminf(top, FLT_MAX);
+    const Weight weight{top, fminf(__double2float_rd(m - S_FAR * t), nextafterf(top, -INFINITY)), m, 369.32993046757463 / t};  // 256 / ln 2
     // where no difference nor quotient that matters leaves the range of 32 bits
     const bool near = fabsf(top) < 1e37f && temp > 1e-30f && temp < 1e30f;
-    S s{cl, full, first, rank, ranks, tid, warp, lane, weight, near, (float)(inv * S_SCALE)};
+    S s{cl, full, first, rank, ranks, tid, warp, lane, weight, near, (float)(S_SCALE / t)};
     const int k = p.top_k ? p.top_k[row] : 0;
     const float top_p = p.top_p ? p.top_p[row] : 1.0f, u = p.u[row];
     double min_w = p.min_p ? (double)p.min_p[row] : 0.0;
@@ -630,15 +637,15 @@ __global__ void __launch_bounds__(S_THREADS, 2) sample_kernel(const sdy_sample_a
             }
             return;
         }
-        cut = s.template find_cut<false>(cut, bound, [&](Sum all) { return min((u64)k, all.count); });
+        cut = s.template find_cut<false>(cut, bound, [&](u64 all) { return min((u64)k, all); });
     }
     if (top_p < 1.0f)
-        cut = s.template find_cut<true>(cut, -FLT_MAX, [&](Sum all) {
-            return max((u64)ceil(max((double)top_p, 0.0) * (double)all.mass), (u64)1);
+        cut = s.template find_cut<true>(cut, -FLT_MAX, [&](u64 all) {
+            return max((u64)ceil(max((double)top_p, 0.0) * (double)all), (u64)1);
         });
     // what is too far for min_p (or for any mass) needs no exponential
-    float low = near ? (float)((double)top - (min_w > 0.0 ? fmin(S_FAR, -log(min_w)) : S_FAR) * 1.001 * (double)temp) : -FLT_MAX;
-    low = fmaxf(low - 1e-5f * fabsf(low), cut.value);
+    float low = __double2float_rd(m - ((min_w > 0.0 ? fmin(S_FAR, -log(min_w)) : S_FAR) * 1.001 + 1e-9) * t);
+    low = fmaxf(low, cut.value);
     u64 total, mass;
     id = s.locate(
         low, INFINITY, cut,
@@ -680,12 +687,20 @@ bool sample_check(const sdy_sample_args *a) {
 
 }  // namespace
 
-// CTAs to a row: as few as hold it, more while that leaves eight to an SM.
+// CTAs to a row: as few as hold it; more while all stay within one to an SM, and, where two would not
+// share an SM, within eight. Measured with 1, 2, 4 and 8 to a row (us): 64 rows of 6000, top-k 40 and
+// top-p, 9.4, 9.3, 11.6, 21.3; 128 rows 9.4, 11.9, 20.2, 35.8; 8 rows of 49152 with filters of all kinds
+// 64, 44, 33, 28; 333 rows of 49152, bf16, 91, 80, 98, 155; 64 rows of 151936, bf16, 98 with 2, 72
+// with 4, 63 with 8.
 template <class T>
 void sample_launch(const sdy_sample_args &a, cudaStream_t s) {
-    constexpr int64_t ROOM = 196 * 1024;  // beside the static shared memory
+    constexpr int64_t ROOM = 196 * 1024, PAIR = 86 * 1024;  // beside the static shared memory: of one CTA in an SM, of two
     int ranks = 1;
-    while (ranks < S_CLUSTER && ((int64_t)(a.n_vocab * sizeof(T)) > ranks * ROOM || (int64_t)a.n_row * ranks * 2 <= 8 * 148)) ranks *= 2;
+    while (ranks < S_CLUSTER) {
+        const int64_t part = (int64_t)(a.n_vocab * sizeof(T)) / ranks;
+        if (part <= ROOM && (int64_t)a.n_row * ranks * 2 > (part > PAIR ? 8 * 148 : 148)) break;
+        ranks *= 2;
+    }
     const int per = ((a.n_vocab + ranks - 1) / ranks + 15) / 16 * 16;
     static std::atomic<uint64_t> done{0};
     smem_limit_once(sample_kernel<T>, (int)ROOM, done);
