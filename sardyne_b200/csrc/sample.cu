@@ -37,7 +37,8 @@ constexpr int S_THREADS = 512, S_WARPS = S_THREADS / 32;
 constexpr int S_MAX_VOCAB = SAMPLE_MAX_VOCAB;
 constexpr int S_CLUSTER = 8;                   // CTAs to a row, at most
 constexpr int S_BUCKETS = 1024, S_LIST = 1024;  // the list: entries ranked at once
-constexpr int S_FEW = 512;                     // a top-k that the first CTA finishes alone, one entry to a thread
+constexpr int S_FEW = 512;                     // a top-k that the first CTA finishes alone, one entry to a thread (1000 so, two to a
+                                               // thread: 41 us against 23 for 12 rows, the sums below quadratic)
 constexpr double S_SCALE = 32.0;               // buckets per unit of (max - l) / T, for numbers of entries
 constexpr int S_STEPS = 16;                    // steps of ln 2 / 256 to a bucket, for masses
 constexpr double S_FAR = 31.3;                 // exp(-31.3) 2^44 < 1/2: no mass from here on

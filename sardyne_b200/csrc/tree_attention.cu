@@ -13,14 +13,21 @@ namespace sdy {
 namespace {
 
 // In 32 bits on the CUDA cores: f32 caches, and 16-bit ones that tree_attention_tc.cu does not take. A
-// CTA holds 16 x RPT rows of one KV head; half-warp y has rows y RPT .., its lane x the keys x, x + 16, ..
-// of a tile of 64 and the elements 4 x .. + 3, 64 + 4 x .., .. of the result, so scores, probabilities
-// and sums of a row stay within its half-warp. K and V tiles come by cp.async, the next ones under this
-// one's products.
+// warp holds RW rows of one KV head; its lanes have a key or two each of a tile of 64 for the scores and
+// hd / 32 elements each of the result, so that all lanes read K and V at different addresses and the
+// rows' Q and probabilities at the same ones (a 16-byte read of shared memory takes a cycle for every
+// eight lanes, whether or not other lanes read the same, and one in all where all do). With WK 2, two
+// warps share their rows and take half a tile's keys each, joined at the end. K and V tiles come by
+// cp.async, the next ones under this one's products.
 //
-// Bound by HBM for few rows, by the 32-bit multiply-adds (2 x 64 x head_dim per row and tile) for many:
-// a thread's RPT x 4 scores take 4 + RPT shared memory reads of 16 bytes per 16 RPT of them.
-constexpr int FK = 64, F_THREADS = 256;
+// Bound by HBM for few rows, by the 32-bit multiply-adds (2 x 64 x head_dim per row and tile) and the
+// reads of shared memory (per 4 elements 4 cycles for a key of each lane, 2 for a row) about equally
+// for many. Measured: 1 token, 32 over 8 heads of 128, 30000 keys 116 us (2.2 TB/s; 168 with half-warps
+// along the keys, whose reads of K and V do not merge), 16 sequences x 4 nodes over 2000 keys 72 us
+// (131), 7 x 52 over 4367 464 us (29 TFLOP/s; 581), 1 token over 701 keys of 3 heads of 64 11 us, most
+// of it the launches and the latencies of one tile and of the join. F_SETUP, the tiles that the rest of
+// a row group takes the time of: with 0, 1, 2 and 6 the second takes 93, 72, 75 and 93 us.
+constexpr int FK = 64, F_WARPS = 8, F_THREADS = 32 * F_WARPS, F_SETUP = 1;
 struct Fp32Layout {
     int rows, ld, stages;  // row stride of Q, K and V in floats
     __host__ __device__ int q() const { return 0; }
@@ -44,26 +51,43 @@ template <class T> __device__ __forceinline__ float4 load4(const T *p) {
     return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
 }
 template <> __device__ __forceinline__ float4 load4(const float *p) { return *(const float4 *)p; }
-template <class T> __device__ __forceinline__ void store_quad(T *out, float4 v, float f) {
-    struct alignas(4 * sizeof(T)) Quad { T v[4]; } q;
-    q.v[0] = from_f32<T>(f == 0.0f ? 0.0f : v.x * f), q.v[1] = from_f32<T>(f == 0.0f ? 0.0f : v.y * f);
-    q.v[2] = from_f32<T>(f == 0.0f ? 0.0f : v.z * f), q.v[3] = from_f32<T>(f == 0.0f ? 0.0f : v.w * f);
-    *(Quad *)out = q;
+template <class T, int N> __device__ __forceinline__ void store_elements(T *out, const float *v, float f) {
+    struct alignas(N * sizeof(T)) Pack { T v[N]; } q;
+#pragma unroll
+    for (int j = 0; j < N; j++) q.v[j] = from_f32<T>(f == 0.0f ? 0.0f : v[j] * f);
+    *(Pack *)out = q;
 }
 
-template <class T, int RPT, int NC>
+template <int N> struct Elements { float v[N]; };  // of a lane: N lane .., and behind four those of the next 128
+template <int N> __device__ __forceinline__ Elements<N> load_elements(const float *p, int lane) {
+    Elements<N> r;
+    if (N == 2) {
+        const float2 a = *(const float2 *)(p + 2 * lane);
+        r.v[0] = a.x, r.v[1] = a.y;
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 a = *(const float4 *)(p + 32 * j + 4 * lane);
+            r.v[j] = a.x, r.v[j + 1] = a.y, r.v[j + 2] = a.z, r.v[j + 3] = a.w;
+        }
+    }
+    return r;
+}
+
+template <class T, int RW, int WK, int NE>
 __global__ void __launch_bounds__(F_THREADS, 1)
     tree_fp32_kernel(const sdy_tree_attention_args p, const Fp32Layout lay, Cut *cuts, float *part_o, float2 *part_ml) {
-    constexpr int R = 16 * RPT;
+    constexpr int KL = 2 / WK, WR = F_WARPS / WK, R = RW * WR;  // keys to a lane, warps along the rows
+    constexpr int EW = NE < 4 ? NE : 4;                         // elements side by side
     __shared__ int64_t scan[F_THREADS / 32 + 8];
     int64_t found[8];
     __shared__ int16_t up[TA_MAX_NODES];
     __shared__ uint32_t path[TA_MAX_NODES][TA_MAX_NODES / 32 + 1];  // the nodes each node sees; 0: padding
     extern __shared__ __align__(16) float mem[];
     pdl_wait();
-    const int tid = threadIdx.x, x = tid % 16, y = tid / 16, hd = p.head_dim, ld = lay.ld;
+    const int tid = threadIdx.x, lane = tid % 32, wr = tid / 32 % WR, wk = tid / 32 / WR, hd = p.head_dim, ld = lay.ld;
     const int rep = p.n_head / p.n_kv_head, rows = p.n_node * rep, groups = (rows + R - 1) / R, items = p.n_kv_head * groups;
-    find_share<FK, F_THREADS>(p, items, blockIdx.x, scan, found);
+    find_share<FK, F_THREADS, F_SETUP>(p, items, blockIdx.x, scan, found);
     if (tid == 0) note_cut<FK>(p, items, groups, blockIdx.x, found, cuts);
     Share<FK> share(p, found, items);
     Segment g;
@@ -74,11 +98,15 @@ __global__ void __launch_bounds__(F_THREADS, 1)
         const int32_t *parent = p.parent ? p.parent + (int64_t)g.s * p.n_node : nullptr;
         const T *kc = (const T *)p.k_cache + g.s * p.cache_seq + g.head * p.cache_head;
         const T *vc = (const T *)p.v_cache + g.s * p.cache_seq + g.head * p.cache_head;
-        const int quads = hd / 4;
+        const int quads = hd / 4, r0 = tid / quads, c0 = tid % quads, dr = F_THREADS / quads, dc = F_THREADS % quads;
         // a tile into stage `st`; rows that do not exist are zero
         auto fetch = [&](int tile, int st) {
-            for (int w = tid; w < FK * quads; w += F_THREADS) {
-                const int r = w / quads, e = 4 * (w - r * quads), j = tile * FK + r;
+            for (int r = r0, c = c0; r < FK; r += dr, c += dc) {
+                if (c >= quads) {
+                    c -= quads;
+                    if (++r >= FK) break;
+                }
+                const int e = 4 * c, j = tile * FK + r;
                 float *k = mem + lay.k(st) + r * ld + e, *v = mem + lay.v(st) + r * ld + e;
                 if (j >= len.keys) {
                     *(float4 *)k = *(float4 *)v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -118,18 +146,15 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                     for (int w = 0; w <= TA_MAX_NODES / 32; w++) path[i][w] = 0;
             }
         }
-        float m[RPT], l[RPT];
-        float4 o[RPT][NC];
-        int node[RPT];
-        bool live[RPT];
+        float m[RW], l[RW];
+        Elements<NE> o[RW];
+        unsigned live = ~0u;  // rows of live nodes, as far as this segment knows
+        auto row_of = [&](int i) { return g.group * R + wr * RW + i; };
 #pragma unroll
-        for (int i = 0; i < RPT; i++) {
-            const int row = g.group * R + y * RPT + i;
-            node[i] = row < rows ? row / rep : -1;
-            live[i] = true;
+        for (int i = 0; i < RW; i++) {
             m[i] = -INFINITY, l[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NC; j++) o[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int j = 0; j < NE; j++) o[i].v[j] = 0.0f;
         }
         for (int t = g.t0; t < g.t1; t++) {
             const int st = lay.stages == 2 ? (t - g.t0) & 1 : 0, j0 = t * FK;
@@ -149,27 +174,27 @@ __global__ void __launch_bounds__(F_THREADS, 1)
             float *V = mem + lay.v(st);
             // drafted rows: which keys a row sees; V of padding nodes is zero, and NaN or infinities of
             // others meet only the rows that see them
-            uint64_t sees[RPT];
+            uint64_t sees[RW];
             bool odd = false;
 #pragma unroll
-            for (int i = 0; i < RPT; i++) sees[i] = ~0ull;
+            for (int i = 0; i < RW; i++) sees[i] = ~0ull;
             if (j0 + FK > len.cached) {
                 const int from = min(max(len.cached - j0, 0), FK), d0 = j0 + from - len.past;  // first drafted row of the tile
                 const int drafted = min(len.keys - j0, FK) - from;
-#pragma unroll
-                for (int i = 0; i < RPT; i++) {
-                    const bool here = node[i] >= 0;
-                    live[i] = here && (path[here ? node[i] : 0][(here ? node[i] : 0) >> 5] >> (node[i] & 31) & 1);
-                    uint64_t bits = 0;
-                    if (live[i] && drafted > 0) {  // bits d0 .. of the path
-                        const uint32_t *w = path[node[i]] + (d0 >> 5);
-                        const int words = TA_MAX_NODES / 32 - (d0 >> 5);  // (the last word is zero)
-                        const uint64_t lo = w[0] | (uint64_t)(words > 1 ? w[1] : 0) << 32, hi = words > 2 ? w[2] : 0;
-                        bits = lo >> (d0 & 31) | ((d0 & 31) ? hi << (64 - (d0 & 31)) : 0);
-                        if (drafted < 64) bits &= (1ull << drafted) - 1;
-                    }
-                    sees[i] = !live[i] ? 0 : from == 64 ? ~0ull : ((1ull << from) - 1) | bits << from;
+                const int row = row_of(lane % RW), node = row < rows ? row / rep : 0;  // a lane finds one row's
+                const bool lives = row < rows && (path[node][node >> 5] >> (node & 31) & 1);
+                uint64_t bits = 0;
+                if (lives && drafted > 0) {  // bits d0 .. of the path
+                    const uint32_t *w = path[node] + (d0 >> 5);
+                    const int words = TA_MAX_NODES / 32 - (d0 >> 5);  // (the last word is zero)
+                    const uint64_t lo = w[0] | (uint64_t)(words > 1 ? w[1] : 0) << 32, hi = words > 2 ? w[2] : 0;
+                    bits = lo >> (d0 & 31) | ((d0 & 31) ? hi << (64 - (d0 & 31)) : 0);
+                    if (drafted < 64) bits &= (1ull << drafted) - 1;
                 }
+                bits = !lives ? 0 : from == 64 ? ~0ull : ((1ull << from) - 1) | bits << from;
+                live = __ballot_sync(~0u, lives);
+#pragma unroll
+                for (int i = 0; i < RW; i++) sees[i] = __shfl_sync(~0u, bits, i);
                 for (int w = tid; w < max(drafted, 0) * quads; w += F_THREADS) {
                     const int r = w / quads, d = d0 + r;
                     float4 *v = (float4 *)(V + (from + r) * ld + 4 * (w - r * quads));
@@ -178,72 +203,68 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                 }
                 odd = __syncthreads_or(odd);
             }
-            float s[RPT][4];
+            float s[RW][KL];
+            const int key = wk * 32 * KL + lane;  // and 32 behind it
 #pragma unroll
-            for (int i = 0; i < RPT; i++)
+            for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[i][j] = 0.0f;
+                for (int j = 0; j < KL; j++) s[i][j] = 0.0f;
 #pragma unroll 4
             for (int e = 0; e < hd; e += 4) {
-                float4 q[RPT], k[4];
+                float4 k[KL];
 #pragma unroll
-                for (int i = 0; i < RPT; i++) q[i] = *(const float4 *)(Q + (y * RPT + i) * ld + e);
+                for (int j = 0; j < KL; j++) k[j] = *(const float4 *)(K + (key + 32 * j) * ld + e);
 #pragma unroll
-                for (int j = 0; j < 4; j++) k[j] = *(const float4 *)(K + (x + 16 * j) * ld + e);
+                for (int i = 0; i < RW; i++) {
+                    const float4 q = *(const float4 *)(Q + (wr * RW + i) * ld + e);
 #pragma unroll
-                for (int i = 0; i < RPT; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        s[i][j] += q[i].x * k[j].x + q[i].y * k[j].y + q[i].z * k[j].z + q[i].w * k[j].w;
+                    for (int j = 0; j < KL; j++) s[i][j] += q.x * k[j].x + q.y * k[j].y + q.z * k[j].z + q.w * k[j].w;
+                }
             }
-            float f[RPT];
+            float f[RW], *own = P + wr * RW * (FK + 4);
 #pragma unroll
-            for (int i = 0; i < RPT; i++) {
+            for (int i = 0; i < RW; i++) {
                 float top = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    s[i][j] = sees[i] >> (x + 16 * j) & 1 ? s[i][j] * c : -INFINITY;
+                for (int j = 0; j < KL; j++) {
+                    s[i][j] = sees[i] >> (key + 32 * j) & 1 ? s[i][j] * c : -INFINITY;
                     top = fmaxf(top, s[i][j]);
                 }
 #pragma unroll
-                for (int b = 8; b; b >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, b));
+                for (int b = 16; b; b >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, b));
                 const float now = fmaxf(m[i], top), off = now == -INFINITY ? 0.0f : now;
                 f[i] = exp2f(m[i] - off);  // (0 at first)
                 m[i] = now;
-                float w[4];
+                l[i] *= f[i];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    w[j] = exp2f(s[i][j] - off);
-                    P[(y * RPT + i) * (FK + 4) + x + 16 * j] = w[j];
+                for (int j = 0; j < KL; j++) {
+                    const float w = exp2f(s[i][j] - off);
+                    own[i * (FK + 4) + key + 32 * j] = w;
+                    l[i] += w;
                 }
-                l[i] = l[i] * f[i] + ((w[0] + w[1]) + (w[2] + w[3]));
             }
             __syncwarp();
             // (a tile's sum on its own, then to the others': a long cache's sums err by its tiles, not its keys)
-            float4 sum[RPT][NC];
+            Elements<NE> sum[RW];
 #pragma unroll
-            for (int i = 0; i < RPT; i++)
+            for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int j = 0; j < NC; j++) sum[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int j = 0; j < NE; j++) sum[i].v[j] = 0.0f;
             auto products = [&](auto skip_zero) {
 #pragma unroll 2
-                for (int k = 0; k < FK; k += 4) {
-                    float4 w[RPT];
+                for (int k = wk * 32 * KL; k < (wk + 1) * 32 * KL; k += 4) {
+                    Elements<NE> v[4];
 #pragma unroll
-                    for (int i = 0; i < RPT; i++) w[i] = *(const float4 *)(P + (y * RPT + i) * (FK + 4) + k);
+                    for (int b = 0; b < 4; b++) v[b] = load_elements<NE>(V + (k + b) * ld, lane);
 #pragma unroll
-                    for (int j = 0; j < NC; j++) {
-                        const int e = 64 * j + 4 * x;
-                        if (e >= hd) continue;
+                    for (int i = 0; i < RW; i++) {
+                        const float4 w4 = *(const float4 *)(own + i * (FK + 4) + k);
+                        const float w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
                         for (int b = 0; b < 4; b++) {
-                            const float4 v = *(const float4 *)(V + (k + b) * ld + e);
+                            if (skip_zero() && w[b] == 0.0f) continue;
 #pragma unroll
-                            for (int i = 0; i < RPT; i++) {
-                                const float a = b == 0 ? w[i].x : b == 1 ? w[i].y : b == 2 ? w[i].z : w[i].w;
-                                if (skip_zero() && a == 0.0f) continue;
-                                sum[i][j].x += a * v.x, sum[i][j].y += a * v.y, sum[i][j].z += a * v.z, sum[i][j].w += a * v.w;
-                            }
+                            for (int j = 0; j < NE; j++) sum[i].v[j] += w[b] * v[b].v[j];
                         }
                     }
                 }
@@ -251,31 +272,53 @@ __global__ void __launch_bounds__(F_THREADS, 1)
             if (odd) products(std::true_type());
             else products(std::false_type());
 #pragma unroll
-            for (int i = 0; i < RPT; i++)
+            for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int j = 0; j < NC; j++) {
-                    o[i][j].x = o[i][j].x * f[i] + sum[i][j].x, o[i][j].y = o[i][j].y * f[i] + sum[i][j].y;
-                    o[i][j].z = o[i][j].z * f[i] + sum[i][j].z, o[i][j].w = o[i][j].w * f[i] + sum[i][j].w;
-                }
+                for (int j = 0; j < NE; j++) o[i].v[j] = o[i].v[j] * f[i] + sum[i].v[j];
             __syncthreads();  // the tile has been read
         }
         const bool whole = g.t0 == 0 && g.t1 == g.tiles;
         const int64_t slot = 2 * blockIdx.x + (seg > 0);
 #pragma unroll
-        for (int i = 0; i < RPT; i++) {
+        for (int i = 0; i < RW; i++)
 #pragma unroll
-            for (int b = 8; b; b >>= 1) l[i] += __shfl_xor_sync(~0u, l[i], b);
-            if (node[i] < 0) continue;
-            const int r = y * RPT + i, row = g.group * R + r;
-            if (!whole && x == 0) part_ml[slot * R + r] = make_float2(m[i], live[i] ? l[i] : -1.0f);
-            T *out = (T *)p.out + g.s * p.out_seq + node[i] * p.out_node + (g.head * rep + row - node[i] * rep) * p.out_head;
+            for (int b = 16; b; b >>= 1) l[i] += __shfl_xor_sync(~0u, l[i], b);
+        if (WK == 2) {  // the second warp's through shared memory (the first stage's, which has been read)
+            float *shared_o = mem + lay.k(0) + wr * RW * 32 * NE, *shared_ml = P + wr * RW * 2;
+            if (wk == 1) {
+#pragma unroll
+                for (int i = 0; i < RW; i++) {
+#pragma unroll
+                    for (int j = 0; j < NE; j++) shared_o[(i * NE + j) * 32 + lane] = o[i].v[j];
+                    if (lane == 0) shared_ml[2 * i] = m[i], shared_ml[2 * i + 1] = l[i];
+                }
+            }
+            __syncthreads();
+            if (wk == 1) continue;
+#pragma unroll
+            for (int i = 0; i < RW; i++) {
+                const float m1 = shared_ml[2 * i], now = fmaxf(m[i], m1), off = now == -INFINITY ? 0.0f : now;
+                const float f0 = exp2f(m[i] - off), f1 = exp2f(m1 - off);
+                m[i] = now, l[i] = l[i] * f0 + shared_ml[2 * i + 1] * f1;
+#pragma unroll
+                for (int j = 0; j < NE; j++) o[i].v[j] = o[i].v[j] * f0 + shared_o[(i * NE + j) * 32 + lane] * f1;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RW; i++) {
+            const int r = wr * RW + i, row = row_of(i), node = row / rep;
+            if (row >= rows) continue;
+            const bool lives = live >> i & 1;
+            if (!whole && lane == 0) part_ml[slot * R + r] = make_float2(m[i], lives ? l[i] : -1.0f);
+            T *out = (T *)p.out + g.s * p.out_seq + node * p.out_node + (g.head * rep + row - node * rep) * p.out_head;
             float *part = part_o + slot * part_stride(R, hd) + (int64_t)r * hd;
+            const float by = lives && l[i] != 0.0f ? 1.0f / l[i] : 0.0f;
 #pragma unroll
-            for (int j = 0; j < NC; j++) {
-                const int e = 64 * j + 4 * x;
+            for (int j = 0; j < NE; j += EW) {
+                const int e = 32 * j + EW * lane;
                 if (e >= hd) continue;
-                if (whole) store_quad(out + e, o[i][j], live[i] && l[i] != 0.0f ? 1.0f / l[i] : 0.0f);
-                else *(float4 *)(part + e) = o[i][j];
+                if (whole) store_elements<T, EW>(out + e, o[i].v + j, by);
+                else store_elements<float, EW>(part + e, o[i].v + j, 1.0f);
             }
         }
     }
@@ -359,7 +402,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS)
                     if (f == 0.0f) v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     acc.x += f * v[c].x, acc.y += f * v[c].y, acc.z += f * v[c].z, acc.w += f * v[c].w;
                 }
-                store_quad(out + d, acc, dead || sum == 0.0f ? 0.0f : 1.0f / sum);
+                store_elements<T, 4>(out + d, &acc.x, dead || sum == 0.0f ? 0.0f : 1.0f / sum);
             }
             continue;
         }
@@ -408,7 +451,7 @@ __global__ void __launch_bounds__(32 * JOIN_WARPS)
                 if (f == 0.0f) continue;  // nothing seen there
                 acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
             }
-            if (real) store_quad(out + d, acc, 1.0f);
+            if (real) store_elements<T, 4>(out + d, &acc.x, 1.0f);
         }
         asm volatile("cp.async.wait_group 0;\n" ::: "memory");
     }
@@ -459,28 +502,28 @@ bool tree_check(const sdy_tree_attention_args *a) {
     return device_pointers(fn, {{"q", a->q}, {"k_cache", a->k_cache}, {"v_cache", a->v_cache}, {"n_past", a->n_past}, {"parent", a->parent}, {"out", a->out}, {"ws", a->ws}});
 }
 
-template <class T, int RPT, int NC>
+template <class T, int RW, int WK, int NE>
 void fp32_launch(const sdy_tree_attention_args &a, const TreeSpace &sp, cudaStream_t s) {
     const Fp32Layout lay = fp32_layout(a);
     static std::atomic<uint64_t> done{0};
-    smem_limit_once(tree_fp32_kernel<T, RPT, NC>, F_SMEM, done);
-    launch(tree_fp32_kernel<T, RPT, NC>, TA_CTAS, F_THREADS, lay.bytes(), s, a, lay, sp.cuts, sp.o, sp.ml);
+    smem_limit_once(tree_fp32_kernel<T, RW, WK, NE>, F_SMEM, done);
+    launch(tree_fp32_kernel<T, RW, WK, NE>, TA_CTAS, F_THREADS, lay.bytes(), s, a, lay, sp.cuts, sp.o, sp.ml);
     SDY_LAUNCHED();
 }
-template <class T, int RPT>
+template <class T, int RW, int WK>
 void fp32_pick(const sdy_tree_attention_args &a, const TreeSpace &sp, cudaStream_t s) {
-    if (a.head_dim <= 64) fp32_launch<T, RPT, 1>(a, sp, s);
-    else if (a.head_dim <= 128) fp32_launch<T, RPT, 2>(a, sp, s);
-    else fp32_launch<T, RPT, 4>(a, sp, s);
+    if (a.head_dim <= 64) fp32_launch<T, RW, WK, 2>(a, sp, s);
+    else if (a.head_dim <= 128) fp32_launch<T, RW, WK, 4>(a, sp, s);
+    else fp32_launch<T, RW, WK, 8>(a, sp, s);
 }
 template <class T>
 void tree_launch(const sdy_tree_attention_args &a, cudaStream_t s) {
     if (tree_tc_takes(a)) return tree_tc(a, s);
     const int rows = fp32_rows(a);
     const TreeSpace sp = tree_space(a, rows);
-    if (rows == 16) fp32_pick<T, 1>(a, sp, s);
-    else if (rows == 32) fp32_pick<T, 2>(a, sp, s);
-    else fp32_pick<T, 4>(a, sp, s);
+    if (rows == 16) fp32_pick<T, 4, 2>(a, sp, s);
+    else if (rows == 32) fp32_pick<T, 8, 2>(a, sp, s);
+    else fp32_pick<T, 8, 1>(a, sp, s);
     tree_join(a, sp, rows, s);
 }
 

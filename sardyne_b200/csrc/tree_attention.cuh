@@ -12,7 +12,7 @@ constexpr int TC_MAX_DIM = 128;  // of the tensor-core kernel
 
 // The split. A row group is the rows (node, query head) of one KV head of one sequence that a CTA
 // holds at once. Its work is its tiles of keys and, unless every tile finds a CTA of its own,
-// TA_SETUP more units for loading the queries and storing the result (about as long as that many
+// SETUP more units for loading the queries and storing the result (about as long as that many
 // tiles, most of the time of a short sequence). The units of a call, sequence
 // by sequence, KV head by KV head, row group by row group, are dealt to TA_CTAS CTAs in equal
 // contiguous shares, whatever the lengths of the sequences, which only the device knows. A CTA
@@ -20,7 +20,6 @@ constexpr int TC_MAX_DIM = 128;  // of the tensor-core kernel
 // the unnormalised sum, the maximum and the sum of weights in one of its two slots of the workspace
 // (first and last row group of its share), and join_kernel adds them up in the order of the CTAs.
 constexpr int TA_CTAS = 148;  // one per SM
-constexpr int TA_SETUP = 6;
 
 // A row group to join, noted by the second CTA that holds tiles of it: the parts are the slot of
 // that CTA's predecessor and the first slots of the CTAs from it on.
@@ -137,7 +136,7 @@ struct Share {
 // Where CTA `cta`'s share begins, for all threads of the block: out[0..7] = first unit, end, first
 // sequence, units before it, its tiles, all units, its length, the setup. Up to 32 sequences are
 // found by every warp for itself; more by a scan over the block's threads, each with a run of sequences.
-template <int KEYS, int THREADS>
+template <int KEYS, int THREADS, int SETUP>
 __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int items, int cta,
                                            int64_t *scan /* shared, THREADS / 32 + 8 */, int64_t (&out)[8]) {
     const int t = threadIdx.x, lane = t % 32;
@@ -151,7 +150,7 @@ __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int
             const int v = __shfl_up_sync(~0u, sum, o);
             if (lane >= o) sum += v;
         }
-        const int total = __shfl_sync(~0u, sum, 31), setup = (int64_t)total * items <= TA_CTAS ? 0 : TA_SETUP;
+        const int total = __shfl_sync(~0u, sum, 31), setup = (int64_t)total * items <= TA_CTAS ? 0 : SETUP;
         const int64_t units = ((int64_t)total + p.n_seq * setup) * items;
         const int64_t u0 = share_begin(units, cta), u1 = share_begin(units, cta + 1);
         const int before = sum - mine + lane * setup;
@@ -180,7 +179,7 @@ __device__ __forceinline__ void find_share(const sdy_tree_attention_args &p, int
         if (w < t / 32) before += scan[w];
         total += scan[w];
     }
-    const int setup = total * items <= TA_CTAS ? 0 : TA_SETUP;
+    const int setup = total * items <= TA_CTAS ? 0 : SETUP;
     before += sum - mine + (int64_t)s0 * setup;
     mine += (int64_t)(s1 - s0) * setup;
     const int64_t units = (total + (int64_t)p.n_seq * setup) * items;

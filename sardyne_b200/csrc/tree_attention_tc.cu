@@ -41,6 +41,7 @@ namespace {
 constexpr int TK = 128;       // keys per tile
 constexpr int TR = 128;       // rows per MMA tile
 constexpr int TT = 384;       // threads
+constexpr int T_SETUP = 6;      // tiles that the rest of a row group takes the time of (3: 72 us for 16 sequences of 24 nodes, 6: 67)
 constexpr int CHUNK = TK * 128, QCHUNK = TR * 128;  // bytes of 64 elements of a tile's rows, 128-byte swizzled
 constexpr int WAIT_LIMIT = 1 << 22;  // mbarrier polls before giving up (about a second)
 // TMEM columns of stream 0's S (and P over it) and O; stream 1's are 128 on.
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(TT, 1)
     }
     pdl_wait();
     int64_t found[8];
-    find_share<TK, TT>(p, p.n_kv_head * groups, blockIdx.x, sh.scan, found);
+    find_share<TK, TT, T_SETUP>(p, p.n_kv_head * groups, blockIdx.x, sh.scan, found);
     fence_before();
     __syncthreads();
     fence_after();
