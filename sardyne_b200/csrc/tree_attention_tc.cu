@@ -41,7 +41,9 @@ namespace {
 constexpr int TK = 128;       // keys per tile
 constexpr int TR = 128;       // rows per MMA tile
 constexpr int TT = 384;       // threads
-constexpr int T_SETUP = 6;      // tiles that the rest of a row group takes the time of (3: 72 us for 16 sequences of 24 nodes, 6: 67)
+// Tiles that the rest of a row group takes the time of: 16 sequences of 24 nodes, up to 8192 keys, and 21 of
+// 13 over up to 5285 take 68.2 and 55.8 us with 3, 62.4 and 48.3 with 6, 63.6 and 47.5 with 9.
+constexpr int T_SETUP = 6;
 constexpr int CHUNK = TK * 128, QCHUNK = TR * 128;  // bytes of 64 elements of a tile's rows, 128-byte swizzled
 constexpr int WAIT_LIMIT = 1 << 22;  // mbarrier polls before giving up (about a second)
 // TMEM columns of stream 0's S (and P over it) and O; stream 1's are 128 on.
