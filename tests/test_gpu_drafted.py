@@ -274,6 +274,18 @@ def test_tree_attention(kind, shape):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", [(2, 20, 4, 2, 256, [130, 7]), (1, 11, 8, 4, 136, [70]), (1, 70, 4, 2, 248, [65]),
+                                   (40, 3, 14, 2, 72, [5 * i for i in range(40)]), (1, 9, 6, 3, 160, [3001])])
+def test_tree_attention_rows_and_wide_heads(kind, shape):
+    """One, two and several groups of rows of heads wider than the tensor cores' tiles; many sequences."""
+    n_seq, nodes, heads, kv, dim, past = shape
+    q, k, v, n_past, parent, par, clean = tree_case(kind, n_seq, nodes, heads, kv, dim, past, seed=5)
+    out = torch.full_like(q, float("nan"))
+    call(capi.lib().sdy_tree_attention_dev, tree_args(kind, q, k, v, n_past, parent, out, dim ** -0.5))
+    check_tree(kind, q, clean, n_past, par, dim ** -0.5, out)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("nodes,heads,kv,past", [(1, 8, 2, 20011), (5, 4, 1, 9001), (24, 8, 2, 5003)])
 def test_tree_attention_long(kind, nodes, heads, kv, past):
     """Long caches, which are split over the keys and joined."""
@@ -481,6 +493,34 @@ def test_sample_filters(kind, vocab):
                      top_p=np.where(r % 4 == 1, 0.5, 1.0), min_p=np.where(r % 5 == 2, 0.02, 0.0))]
     for s in settings:
         check_sample(x, u, sample(x, u, kind, **s), **s)
+
+
+@pytest.mark.parametrize("kind,rows,vocab", [("f32", 20, 1500), ("f16", 40, 1500), ("bf16", 160, 1500), ("f32", 160, 9001),
+                                             ("bf16", 80, 60001), ("f32", 30, 70001)])
+def test_sample_many_rows(kind, rows, vocab):
+    """Rows enough that each has one CTA, two or four."""
+    g = gen(rows + vocab)
+    x = (randn(g, rows, vocab) * 3).to(DTYPE[kind])
+    x[::3, ::2] = -float("inf")
+    u = torch.rand(rows, generator=g, device="cuda").cpu().numpy()
+    r = np.arange(rows)
+    s = dict(temperature=np.where(r % 7 == 6, 0.0, 0.5 + r % 5 / 4), top_k=np.select([r % 6 == 1, r % 6 == 3, r % 6 == 4], [40, 900, 600]),
+             top_p=np.where((r % 6 == 2) | (r % 6 == 3), 0.9, 1.0), min_p=np.where(r % 6 == 5, 0.05, 0.0))
+    check_sample(x, u, sample(x, u, kind, **s), **s)
+    check_sample(x[:, 1:], u, sample(x[:, 1:], u, kind, top_p=0.95), top_p=0.95)
+
+
+@pytest.mark.parametrize("temperature", [1e-40, 1e-30, 1e-3, 1e20, 3e38])
+@pytest.mark.parametrize("span", [1e-30, 1.0, 3e38])
+def test_sample_ranges(temperature, span):
+    """Temperatures and logits from one end of the type to the other."""
+    g = gen(31)
+    x = (torch.rand(3, 2000, generator=g, device="cuda") * 2 - 1) * span
+    x[1] = x[1].abs()
+    x[2, 100:] = x[2, 7]
+    u = np.array([0.3, 0.6, 0.9], np.float32)
+    for s in (dict(), dict(top_k=30), dict(top_k=700), dict(top_p=0.6), dict(min_p=0.7), dict(min_p=1.0)):
+        check_sample(x, u, sample(x, u, temperature=temperature, **s), temperature=temperature, **s)
 
 
 @pytest.mark.parametrize("kind", KINDS)
