@@ -327,11 +327,14 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 // The results of the row groups that the shares cut: out = sum_c f_c o_c / sum_c f_c l_c over the
 // CTAs that hold tiles of the group, in their order, with f_c = 2^(m_c - max m). A warp takes one row
 // of a cut group (two or four where rows are narrow), the warps of all SMs in turn: its lanes start the
-// copies of the first sixteen parts into shared memory (as many loads into registers the compiler
+// copies of the first eight parts into shared memory (as many loads into registers the compiler
 // would not keep in flight), form the factors meanwhile, and add up four elements of a row each.
 // Bound by the latencies of the cuts, the maxima and the parts, one after the other (about 1 us each
 // on B200), and for many wide parts by what an SM reads from L2, 64 bytes a cycle.
-constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 16, JOIN_BLOCKS = 5 * TA_CTAS;
+// Both kernels of 16 sequences of 24 nodes, up to 8192 keys: 57.6 us with eight parts ahead and six CTAs
+// to an SM, 59 with eight and four, 58.9 with sixteen and four, 62.4 with sixteen and five (of which one
+// waits for room).
+constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 8, JOIN_BLOCKS = 6 * TA_CTAS;
 constexpr int JOIN_FEW = 4;  // so many parts at most are loaded straight into registers
 constexpr int JOIN_RUNS = (TA_CTAS + 31) / 32;  // cuts, or parts, a lane looks at
 template <class T>
