@@ -22,11 +22,12 @@ namespace {
 //
 // Bound by HBM for few rows, by the 32-bit multiply-adds (2 x 64 x head_dim per row and tile) and the
 // reads of shared memory (per 4 elements 4 cycles for a key of each lane, 2 for a row) about equally
-// for many. Measured: 1 token, 32 over 8 heads of 128, 30000 keys 116 us (2.2 TB/s; 168 with half-warps
-// along the keys, whose reads of K and V do not merge), 16 sequences x 4 nodes over 2000 keys 72 us
-// (131), 7 x 52 over 4367 464 us (29 TFLOP/s; 581), 1 token over 701 keys of 3 heads of 64 11 us, most
-// of it the launches and the latencies of one tile and of the join. F_SETUP, the tiles that the rest of
-// a row group takes the time of: with 0, 1, 2 and 6 the second takes 93, 72, 75 and 93 us.
+// for many. Measured: 1 token, 32 over 8 heads of 128, 30000 keys 92 us (2.7 TB/s; 168 with half-warps
+// along the keys, whose reads of K and V do not merge, 115 with 16 rows to a group instead of 8), 16
+// sequences x 4 nodes over 2000 keys 57 us, 3 x 5 over 45953, 40 rows, 232 us (286 with groups of 64),
+// 7 x 52 over 4367 461 us (29 TFLOP/s), 1 token over 701 keys of 3 heads of 64 9.4 us, most of it the
+// launches and the latencies of one tile and of the join. F_SETUP, the tiles that the rest of a row
+// group takes the time of: with 0, 1, 2 and 6 the second took 93, 72, 75 and 93 us in groups of 16.
 constexpr int FK = 64, F_WARPS = 8, F_THREADS = 32 * F_WARPS, F_SETUP = 1;
 struct Fp32Layout {
     int rows, ld, stages;  // row stride of Q, K and V in floats
@@ -37,9 +38,16 @@ struct Fp32Layout {
     __host__ __device__ int bytes() const { return (p() + rows * (FK + 4)) * 4; }
 };
 constexpr int F_SMEM = 217 * 1024;  // beside the static shared memory
+// Rows to a group: those whose groups read least of shared memory in all (cycles per tile and group, for
+// heads of 128).
 inline int fp32_rows(const sdy_tree_attention_args &a) {
+    static const int size[5] = {64, 48, 32, 16, 8}, cost[5] = {10200, 8700, 7200, 4600, 3300};
     const int rows = a.n_node * (a.n_head / a.n_kv_head);
-    return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    auto all = [&](int i) { return cost[i] * ((rows + size[i] - 1) / size[i]); };
+    int best = 0;
+    for (int i = 1; i < 5; i++)
+        if (all(i) < all(best)) best = i;
+    return size[best];
 }
 inline Fp32Layout fp32_layout(const sdy_tree_attention_args &a) {
     Fp32Layout l = {fp32_rows(a), a.head_dim + 4, 2};
@@ -524,8 +532,10 @@ void tree_launch(const sdy_tree_attention_args &a, cudaStream_t s) {
     if (tree_tc_takes(a)) return tree_tc(a, s);
     const int rows = fp32_rows(a);
     const TreeSpace sp = tree_space(a, rows);
-    if (rows == 16) fp32_pick<T, 4, 2>(a, sp, s);
+    if (rows == 8) fp32_pick<T, 2, 2>(a, sp, s);
+    else if (rows == 16) fp32_pick<T, 4, 2>(a, sp, s);
     else if (rows == 32) fp32_pick<T, 8, 2>(a, sp, s);
+    else if (rows == 48) fp32_pick<T, 6, 1>(a, sp, s);
     else fp32_pick<T, 8, 1>(a, sp, s);
     tree_join(a, sp, rows, s);
 }
