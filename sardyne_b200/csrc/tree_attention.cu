@@ -14,16 +14,18 @@ namespace {
 
 // In 32 bits on the CUDA cores: f32 caches, and 16-bit ones that tree_attention_tc.cu does not take. A
 // warp holds RW rows of one KV head; its lanes have a key or two each of a tile of 64 for the scores and
-// hd / 32 elements each of the result, so that all lanes read K and V at different addresses and the
-// rows' Q and probabilities at the same ones (a 16-byte read of shared memory takes a cycle for every
-// eight lanes, whether or not other lanes read the same, and one in all where all do). With WK 2, two
-// warps share their rows and take half a tile's keys each, joined at the end. K and V tiles come by
-// cp.async, the next ones under this one's products.
+// hd / 32 elements each of the result, so that all lanes read K and V at different addresses (a 16-byte
+// read of shared memory takes a cycle for every eight lanes, whether or not other lanes read the same)
+// and the rows' Q and probabilities at the same one. With WK 2, two warps share their rows and take
+// half a tile's keys each, joined at the end. K and V tiles come by cp.async, the next ones under this
+// one's products.
 //
-// Bound by HBM for few rows, by the 32-bit multiply-adds (2 x 64 x head_dim per row and tile) and the
-// reads of shared memory (per 4 elements 4 cycles for a key of each lane, 2 for a row) about equally
-// for many. Measured: 1 token, 32 over 8 heads of 128, 30000 keys 92 us (2.7 TB/s; 168 with half-warps
-// along the keys, whose reads of K and V do not merge, 115 with 16 rows to a group instead of 8), 16
+// Bound by HBM and latency for few rows; for many by the reads of shared memory (per 4 elements 4
+// cycles for the keys of a warp's lanes, and 2 to 4 for each row), then the 32-bit multiply-adds (2 x 64 x
+// head_dim per row and tile): a tile of 64 rows of 128 takes 17800 cycles, 8300 the scores, 1000 the softmax,
+// 6600 the sums and 2000 to send for the next tile and wait, against 8200 of multiply-adds. Measured: 1
+// token, 32 over 8 heads of 128, 30000 keys 92 us (2.7 TB/s; 168 with half-warps along the keys, whose
+// reads of K and V do not merge, 115 with 16 rows to a group instead of 8), 16
 // sequences x 4 nodes over 2000 keys 57 us, 3 x 5 over 45953, 40 rows, 232 us (286 with groups of 64),
 // 7 x 52 over 4367 461 us (29 TFLOP/s), 1 token over 701 keys of 3 heads of 64 9.4 us, most of it the
 // launches and the latencies of one tile and of the join. F_SETUP, the tiles that the rest of a row
@@ -38,8 +40,8 @@ struct Fp32Layout {
     __host__ __device__ int bytes() const { return (p() + rows * (FK + 4)) * 4; }
 };
 constexpr int F_SMEM = 217 * 1024;  // beside the static shared memory
-// Rows to a group: those whose groups read least of shared memory in all (cycles per tile and group, for
-// heads of 128).
+// Rows to a group: those whose groups take the least time for a tile in all (about so many cycles of
+// shared memory for heads of 128).
 inline int fp32_rows(const sdy_tree_attention_args &a) {
     static const int size[5] = {64, 48, 32, 16, 8}, cost[5] = {10200, 8700, 7200, 4600, 3300};
     const int rows = a.n_node * (a.n_head / a.n_kv_head);
