@@ -13,23 +13,22 @@ namespace sdy {
 namespace {
 
 // In 32 bits on the CUDA cores: f32 caches, and 16-bit ones that tree_attention_tc.cu does not take. A
-// warp holds RW rows of one KV head; its lanes have a key or two each of a tile of 64 for the scores and
-// hd / 32 elements each of the result, so that all lanes read K and V at different addresses (a 16-byte
-// read of shared memory takes a cycle for every eight lanes, whether or not other lanes read the same)
-// and the rows' Q and probabilities at the same one. With WK 2, two warps share their rows and take
-// half a tile's keys each, joined at the end. K and V tiles come by cp.async, the next ones under this
-// one's products.
+// warp holds RW rows of one KV head and takes the 64 keys of a tile, or with WK 2 half of them, the
+// other half by a second warp and joined at the end. For the scores its halves take every other four
+// elements, their 16 lanes two or four keys each; for the result they take every other four keys,
+// their lanes hd / 16 elements each. A 16-byte read of shared memory takes four cycles for a warp, or
+// little less where lanes read the same, so what counts is how many there are: per 8 elements 2 or 4 for
+// K and one for a row's Q, per 8 keys hd / 16 for V and one for a row's probabilities. K and V tiles
+// come by cp.async, the next ones under this one's products.
 //
-// Bound by HBM and latency for few rows; for many by the reads of shared memory (per 4 elements 4
-// cycles for the keys of a warp's lanes, and 2 to 4 for each row), then the 32-bit multiply-adds (2 x 64 x
-// head_dim per row and tile): a tile of 64 rows of 128 takes 17800 cycles, 8300 the scores, 1000 the softmax,
-// 6600 the sums and 2000 to send for the next tile and wait, against 8200 of multiply-adds. Measured: 1
-// token, 32 over 8 heads of 128, 30000 keys 92 us (2.7 TB/s; 168 with half-warps along the keys, whose
-// reads of K and V do not merge, 115 with 16 rows to a group instead of 8), 16
-// sequences x 4 nodes over 2000 keys 57 us, 3 x 5 over 45953, 40 rows, 232 us (286 with groups of 64),
-// 7 x 52 over 4367 461 us (29 TFLOP/s), 1 token over 701 keys of 3 heads of 64 9.4 us, most of it the
-// launches and the latencies of one tile and of the join. F_SETUP, the tiles that the rest of a row
-// group takes the time of: with 0, 1, 2 and 6 the second took 93, 72, 75 and 93 us in groups of 16.
+// Bound by HBM and latency for few rows; for many by those reads (a tile of 64 rows of 128: 10200 cycles),
+// then the 32-bit multiply-adds (2 x 64 x head_dim per row and tile: 8200); the softmax takes 1000 and to send
+// for the next tile and wait 2000. Measured: 1 token, 32 over 8 heads of 128, 30000 keys 89 us (2.8
+// TB/s; 115 with 16 rows to a group instead of 8), 16 sequences x 4 nodes over 2000 keys 55 us, 3 x 5 over
+// 45953, 40 rows, 214 us (232 with whole warps at the same four elements, 286 in groups of 64), 7 x 52 over
+// 4367 428 us (31 TFLOP/s; 461), 1 token over 701 keys of 3 heads of 64 9.4 us, most of it the launches
+// and the latencies of one tile and of the join. F_SETUP, the tiles that the rest of a row group
+// takes the time of: with 0, 1, 2 and 6 the second took 93, 72, 75 and 93 us in groups of 16.
 constexpr int FK = 64, F_WARPS = 8, F_THREADS = 32 * F_WARPS, F_SETUP = 1;
 struct Fp32Layout {
     int rows, ld, stages;  // row stride of Q, K and V in floats
@@ -46,8 +45,8 @@ inline int fp32_rows(const sdy_tree_attention_args &a) {
     static const int size[5] = {64, 48, 32, 16, 8}, cost[5] = {10200, 8700, 7200, 4600, 3300};
     const int rows = a.n_node * (a.n_head / a.n_kv_head);
     auto all = [&](int i) { return cost[i] * ((rows + size[i] - 1) / size[i]); };
-    int best = 0;
-    for (int i = 1; i < 5; i++)
+    int best = a.head_dim > 128 ? 2 : 0;  // (wider heads: 32 at most, for the registers)
+    for (int i = best + 1; i < 5; i++)
         if (all(i) < all(best)) best = i;
     return size[best];
 }
@@ -68,18 +67,13 @@ template <class T, int N> __device__ __forceinline__ void store_elements(T *out,
     *(Pack *)out = q;
 }
 
-template <int N> struct Elements { float v[N]; };  // of a lane: N lane .., and behind four those of the next 128
-template <int N> __device__ __forceinline__ Elements<N> load_elements(const float *p, int lane) {
+template <int N> struct Elements { float v[N]; };  // of one of 16 lanes: 4 x .. + 3, 64 + 4 x .. + 3, ..
+template <int N> __device__ __forceinline__ Elements<N> load_elements(const float *p, int x) {
     Elements<N> r;
-    if (N == 2) {
-        const float2 a = *(const float2 *)(p + 2 * lane);
-        r.v[0] = a.x, r.v[1] = a.y;
-    } else {
 #pragma unroll
-        for (int j = 0; j < N; j += 4) {
-            const float4 a = *(const float4 *)(p + 32 * j + 4 * lane);
-            r.v[j] = a.x, r.v[j + 1] = a.y, r.v[j + 2] = a.z, r.v[j + 3] = a.w;
-        }
+    for (int j = 0; j < N; j += 4) {
+        const float4 a = *(const float4 *)(p + 16 * j + 4 * x);
+        r.v[j] = a.x, r.v[j + 1] = a.y, r.v[j + 2] = a.z, r.v[j + 3] = a.w;
     }
     return r;
 }
@@ -88,14 +82,14 @@ template <class T, int RW, int WK, int NE>
 __global__ void __launch_bounds__(F_THREADS, 1)
     tree_fp32_kernel(const sdy_tree_attention_args p, const Fp32Layout lay, Cut *cuts, float *part_o, float2 *part_ml) {
     constexpr int KL = 2 / WK, WR = F_WARPS / WK, R = RW * WR;  // keys to a lane, warps along the rows
-    constexpr int EW = NE < 4 ? NE : 4;                         // elements side by side
+    constexpr int EW = NE < 4 ? NE : 4, NL = 2 * NE;            // elements side by side; a lane's while halves differ
     __shared__ int64_t scan[F_THREADS / 32 + 8];
     int64_t found[8];
     __shared__ int16_t up[TA_MAX_NODES];
     __shared__ uint32_t path[TA_MAX_NODES][TA_MAX_NODES / 32 + 1];  // the nodes each node sees; 0: padding
     extern __shared__ __align__(16) float mem[];
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid % 32, wr = tid / 32 % WR, wk = tid / 32 / WR, hd = p.head_dim, ld = lay.ld;
+    const int tid = threadIdx.x, lane = tid % 32, x = lane % 16, half = lane / 16, wr = tid / 32 % WR, wk = tid / 32 / WR, hd = p.head_dim, ld = lay.ld;
     const int rep = p.n_head / p.n_kv_head, rows = p.n_node * rep, groups = (rows + R - 1) / R, items = p.n_kv_head * groups;
     find_share<FK, F_THREADS, F_SETUP>(p, items, blockIdx.x, scan, found);
     if (tid == 0) note_cut<FK>(p, items, groups, blockIdx.x, found, cuts);
@@ -157,14 +151,14 @@ __global__ void __launch_bounds__(F_THREADS, 1)
             }
         }
         float m[RW], l[RW];
-        Elements<NE> o[RW];
+        Elements<NL> o[RW];  // of the half's keys
         unsigned live = ~0u;  // rows of live nodes, as far as this segment knows
         auto row_of = [&](int i) { return g.group * R + wr * RW + i; };
 #pragma unroll
         for (int i = 0; i < RW; i++) {
             m[i] = -INFINITY, l[i] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < NE; j++) o[i].v[j] = 0.0f;
+            for (int j = 0; j < NL; j++) o[i].v[j] = 0.0f;
         }
         for (int t = g.t0; t < g.t1; t++) {
             const int st = lay.stages == 2 ? (t - g.t0) & 1 : 0, j0 = t * FK;
@@ -213,31 +207,37 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                 }
                 odd = __syncthreads_or(odd);
             }
-            float s[RW][KL];
-            const int key = wk * 32 * KL + lane;  // and 32 behind it
+            // each half of the warp takes every other four elements of all the warp's keys, then half the keys
+            const int k0 = wk * 32 * KL, key = k0 + x + half * 16 * KL;  // (and 16 behind it)
+            float part[RW][2 * KL], s[RW][KL];
 #pragma unroll
             for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int j = 0; j < KL; j++) s[i][j] = 0.0f;
-#pragma unroll 4
-            for (int e = 0; e < hd; e += 4) {
-                float4 k[KL];
+                for (int j = 0; j < 2 * KL; j++) part[i][j] = 0.0f;
+#pragma unroll 2
+            for (int e = 4 * half; e < hd; e += 8) {
+                float4 k[2 * KL];
 #pragma unroll
-                for (int j = 0; j < KL; j++) k[j] = *(const float4 *)(K + (key + 32 * j) * ld + e);
+                for (int j = 0; j < 2 * KL; j++) k[j] = *(const float4 *)(K + (k0 + x + 16 * j) * ld + e);
 #pragma unroll
                 for (int i = 0; i < RW; i++) {
                     const float4 q = *(const float4 *)(Q + (wr * RW + i) * ld + e);
 #pragma unroll
-                    for (int j = 0; j < KL; j++) s[i][j] += q.x * k[j].x + q.y * k[j].y + q.z * k[j].z + q.w * k[j].w;
+                    for (int j = 0; j < 2 * KL; j++) part[i][j] += q.x * k[j].x + q.y * k[j].y + q.z * k[j].z + q.w * k[j].w;
                 }
             }
+#pragma unroll
+            for (int i = 0; i < RW; i++)
+#pragma unroll
+                for (int j = 0; j < KL; j++)
+                    s[i][j] = (half ? part[i][KL + j] : part[i][j]) + __shfl_xor_sync(~0u, half ? part[i][j] : part[i][KL + j], 16);
             float f[RW], *own = P + wr * RW * (FK + 4);
 #pragma unroll
             for (int i = 0; i < RW; i++) {
                 float top = -INFINITY;
 #pragma unroll
                 for (int j = 0; j < KL; j++) {
-                    s[i][j] = sees[i] >> (key + 32 * j) & 1 ? s[i][j] * c : -INFINITY;
+                    s[i][j] = sees[i] >> (key + 16 * j) & 1 ? s[i][j] * c : -INFINITY;
                     top = fmaxf(top, s[i][j]);
                 }
 #pragma unroll
@@ -249,23 +249,23 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 #pragma unroll
                 for (int j = 0; j < KL; j++) {
                     const float w = exp2f(s[i][j] - off);
-                    own[i * (FK + 4) + key + 32 * j] = w;
+                    own[i * (FK + 4) + key + 16 * j] = w;
                     l[i] += w;
                 }
             }
             __syncwarp();
             // (a tile's sum on its own, then to the others': a long cache's sums err by its tiles, not its keys)
-            Elements<NE> sum[RW];
+            Elements<NL> sum[RW];
 #pragma unroll
             for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int j = 0; j < NE; j++) sum[i].v[j] = 0.0f;
+                for (int j = 0; j < NL; j++) sum[i].v[j] = 0.0f;
             auto products = [&](auto skip_zero) {
 #pragma unroll 2
-                for (int k = wk * 32 * KL; k < (wk + 1) * 32 * KL; k += 4) {
-                    Elements<NE> v[4];
+                for (int k = k0 + 4 * half; k < k0 + 32 * KL; k += 8) {
+                    Elements<NL> v[4];
 #pragma unroll
-                    for (int b = 0; b < 4; b++) v[b] = load_elements<NE>(V + (k + b) * ld, lane);
+                    for (int b = 0; b < 4; b++) v[b] = load_elements<NL>(V + (k + b) * ld, x);
 #pragma unroll
                     for (int i = 0; i < RW; i++) {
                         const float4 w4 = *(const float4 *)(own + i * (FK + 4) + k);
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                         for (int b = 0; b < 4; b++) {
                             if (skip_zero() && w[b] == 0.0f) continue;
 #pragma unroll
-                            for (int j = 0; j < NE; j++) sum[i].v[j] += w[b] * v[b].v[j];
+                            for (int j = 0; j < NL; j++) sum[i].v[j] += w[b] * v[b].v[j];
                         }
                     }
                 }
@@ -284,22 +284,30 @@ __global__ void __launch_bounds__(F_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < RW; i++)
 #pragma unroll
-                for (int j = 0; j < NE; j++) o[i].v[j] = o[i].v[j] * f[i] + sum[i].v[j];
+                for (int j = 0; j < NL; j++) o[i].v[j] = o[i].v[j] * f[i] + sum[i].v[j];
             __syncthreads();  // the tile has been read
         }
         const bool whole = g.t0 == 0 && g.t1 == g.tiles;
         const int64_t slot = 2 * blockIdx.x + (seg > 0);
+        Elements<NE> sum[RW];
 #pragma unroll
-        for (int i = 0; i < RW; i++)
+        for (int i = 0; i < RW; i++) {
 #pragma unroll
             for (int b = 16; b; b >>= 1) l[i] += __shfl_xor_sync(~0u, l[i], b);
+            // both halves' keys, of half the elements each
+#pragma unroll
+            for (int j = 0; j < NE; j++) {
+                const int a = j / EW * 2 * EW + j % EW;
+                sum[i].v[j] = (half ? o[i].v[a + EW] : o[i].v[a]) + __shfl_xor_sync(~0u, half ? o[i].v[a] : o[i].v[a + EW], 16);
+            }
+        }
         if (WK == 2) {  // the second warp's through shared memory (the first stage's, which has been read)
             float *shared_o = mem + lay.k(0) + wr * RW * 32 * NE, *shared_ml = P + wr * RW * 2;
             if (wk == 1) {
 #pragma unroll
                 for (int i = 0; i < RW; i++) {
 #pragma unroll
-                    for (int j = 0; j < NE; j++) shared_o[(i * NE + j) * 32 + lane] = o[i].v[j];
+                    for (int j = 0; j < NE; j++) shared_o[(i * NE + j) * 32 + lane] = sum[i].v[j];
                     if (lane == 0) shared_ml[2 * i] = m[i], shared_ml[2 * i + 1] = l[i];
                 }
             }
@@ -311,7 +319,7 @@ __global__ void __launch_bounds__(F_THREADS, 1)
                 const float f0 = exp2f(m[i] - off), f1 = exp2f(m1 - off);
                 m[i] = now, l[i] = l[i] * f0 + shared_ml[2 * i + 1] * f1;
 #pragma unroll
-                for (int j = 0; j < NE; j++) o[i].v[j] = o[i].v[j] * f0 + shared_o[(i * NE + j) * 32 + lane] * f1;
+                for (int j = 0; j < NE; j++) sum[i].v[j] = sum[i].v[j] * f0 + shared_o[(i * NE + j) * 32 + lane] * f1;
             }
         }
 #pragma unroll
@@ -325,10 +333,10 @@ __global__ void __launch_bounds__(F_THREADS, 1)
             const float by = lives && l[i] != 0.0f ? 1.0f / l[i] : 0.0f;
 #pragma unroll
             for (int j = 0; j < NE; j += EW) {
-                const int e = 32 * j + EW * lane;
+                const int e = NE < 4 ? 4 * x + 2 * half : 32 * j + 4 * lane;
                 if (e >= hd) continue;
-                if (whole) store_elements<T, EW>(out + e, o[i].v + j, by);
-                else store_elements<float, EW>(part + e, o[i].v + j, 1.0f);
+                if (whole) store_elements<T, EW>(out + e, sum[i].v + j, by);
+                else store_elements<float, EW>(part + e, sum[i].v + j, 1.0f);
             }
         }
     }
@@ -526,15 +534,18 @@ void fp32_launch(const sdy_tree_attention_args &a, const TreeSpace &sp, cudaStre
 template <class T, int RW, int WK>
 void fp32_pick(const sdy_tree_attention_args &a, const TreeSpace &sp, cudaStream_t s) {
     if (a.head_dim <= 64) fp32_launch<T, RW, WK, 2>(a, sp, s);
-    else if (a.head_dim <= 128) fp32_launch<T, RW, WK, 4>(a, sp, s);
-    else fp32_launch<T, RW, WK, 8>(a, sp, s);
+    else fp32_launch<T, RW, WK, 4>(a, sp, s);
 }
 template <class T>
 void tree_launch(const sdy_tree_attention_args &a, cudaStream_t s) {
     if (tree_tc_takes(a)) return tree_tc(a, s);
     const int rows = fp32_rows(a);
     const TreeSpace sp = tree_space(a, rows);
-    if (rows == 8) fp32_pick<T, 2, 2>(a, sp, s);
+    if (a.head_dim > 128) {
+        if (rows == 8) fp32_launch<T, 2, 2, 8>(a, sp, s);
+        else if (rows == 16) fp32_launch<T, 4, 2, 8>(a, sp, s);
+        else fp32_launch<T, 4, 1, 8>(a, sp, s);
+    } else if (rows == 8) fp32_pick<T, 2, 2>(a, sp, s);
     else if (rows == 16) fp32_pick<T, 4, 2>(a, sp, s);
     else if (rows == 32) fp32_pick<T, 8, 2>(a, sp, s);
     else if (rows == 48) fp32_pick<T, 6, 1>(a, sp, s);
